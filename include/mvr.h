@@ -666,6 +666,117 @@ int mvr_normalize_rows(mvr_ctx* ctx, float* rows, uint64_t n_floats, uint32_t di
 /* The same on a device buffer, ordered on the context's stream. */
 int mvr_normalize_rows_device(mvr_ctx* ctx, float* d_rows, uint64_t n_floats, uint32_t dim);
 
+/* ------------------------------------------------------------------------
+ * Token operators (no reference counterpart): a table read by token id with
+ * scaling and its gradient by sorted tokens; rows sorted by group (an expert,
+ * a centroid, a token id) and back, with weights applied, and the gradients.
+ *
+ * All pointers except the `bytes` outputs are device pointers; the calls
+ * enqueue on the context's stream and return without waiting. They use no
+ * scratch of the context: what a call needs beside its inputs and outputs is
+ * the caller's `workspace` (16-byte aligned, contents need not be set or
+ * kept), so calls on different streams or captured graphs do not meet as long
+ * as their workspaces differ. Inputs and outputs of a call must not overlap.
+ *
+ * Rows have `dim` elements of one type (mvr_dtype), consecutive inside a row;
+ * `*_stride` is the distance of two rows in elements (at least dim for
+ * outputs, any value for inputs: 0 repeats one row). Scales and weights are
+ * f32. Sums and products are formed in f32 and rounded once to the element
+ * type. Results do not depend on the launch: the order of every sum is fixed
+ * by the sizes.
+ *
+ * Ids are 4-byte (id_bytes = 4) or 8-byte integers. An id outside [0, rows),
+ * a negative one among them, names no row (padding, a dropped choice): its
+ * lookup is a row of zeros, it takes part in no sum and its gradients are 0.
+ *
+ * Refused with MVR_E_INVALID_ARGUMENT: null pointers where data is needed,
+ * unknown types, strides of outputs below dim, pointers that are not aligned
+ * to their element type, rows == 0, rows >= 2^31 - 1, more than 2^31 - 1 ids
+ * (plan and what uses one), a workspace below the size asked for; with
+ * MVR_E_DIM_MISMATCH: dim == 0.
+ * ------------------------------------------------------------------------ */
+
+enum mvr_dtype { MVR_F32 = 0, MVR_BF16 = 1, MVR_F16 = 2 };
+
+/* Slot of a pair whose id names no row. */
+#define MVR_NO_SLOT 0xFFFFFFFFu
+
+/* out[i] = (alpha * scale[i]) * table[ids[i]] for n ids (scale may be NULL:
+ * ones). table: rows x dim, out: n x dim, both of type `dtype`. */
+int mvr_lookup_device(mvr_ctx* ctx, const void* d_table, int dtype, uint64_t rows, uint32_t dim,
+                      uint64_t table_stride, const void* d_ids, int id_bytes, uint64_t n, const float* d_scale,
+                      float alpha, void* d_out, uint64_t out_stride);
+
+/* Workspace of mvr_token_plan_device for n_ids ids. */
+int mvr_token_plan_bytes(uint64_t n_ids, uint64_t rows, uint64_t* bytes);
+
+/* The stable sort of the ids that name a row (host-visible as CSR):
+ *   offsets[v]  first sorted place of id v (rows + 1 entries); offsets[rows]
+ *               is the number of ids that name a row
+ *   order[p]    the id at sorted place p (ascending inside one v), n_ids
+ *               entries; those at and after offsets[rows] are undefined
+ *   keys[p]     the value v at sorted place p, n_ids entries; at and after
+ *               offsets[rows] they are `rows`
+ *   slot[i]     the sorted place of id i, MVR_NO_SLOT where it names no row;
+ *               n_ids entries */
+int mvr_token_plan_device(mvr_ctx* ctx, const void* d_ids, int id_bytes, uint64_t n_ids, uint64_t rows,
+                          uint32_t* d_offsets, uint32_t* d_order, uint32_t* d_keys, uint32_t* d_slot,
+                          void* d_workspace, uint64_t workspace_bytes);
+
+/* Workspace of mvr_lookup_grad_device. */
+int mvr_lookup_grad_bytes(uint64_t n_ids, uint32_t dim, uint64_t* bytes);
+
+/* Gradients of mvr_lookup_device for the output gradient `grad` (n_ids x dim,
+ * `dtype`), with the plan of its ids:
+ *   dtable[v] = sum over the ids i of v of alpha * scale[i] * grad[i]
+ *   dscale[i] = alpha * dot(grad[i], table[ids[i]])
+ * dtable: rows x dim of type dtable_dtype (`dtype` or MVR_F32); rows without
+ * an id become 0. With accumulate != 0 the sums are added to what dtable
+ * holds and rows without an id are left as they are. dscale (n_ids f32) is
+ * written where it is not NULL; `table` (type `dtype`) is read for it alone
+ * and may be NULL otherwise. */
+int mvr_lookup_grad_device(mvr_ctx* ctx, const void* d_grad, int dtype, uint64_t grad_stride, uint64_t n_ids,
+                           uint64_t rows, uint32_t dim, const uint32_t* d_offsets, const uint32_t* d_order,
+                           const uint32_t* d_keys, const uint32_t* d_slot, const float* d_scale, float alpha,
+                           const void* d_table, uint64_t table_stride, void* d_dtable, int dtable_dtype,
+                           uint64_t dtable_stride, int accumulate, float* d_dscale, void* d_workspace,
+                           uint64_t workspace_bytes);
+
+/* Rows into sorted order. Each of n tokens has `columns` ids; slot is that of
+ * the plan of the n x columns ids, weights n x columns (NULL: ones):
+ *   out[slot[i, c]] = weights[i, c] * x[i]
+ * x: n x dim; out: n * columns rows, of which those behind the last sorted
+ * row are left as they are. */
+int mvr_group_rows_device(mvr_ctx* ctx, const void* d_x, int dtype, uint64_t x_stride, uint64_t n, uint32_t columns,
+                          uint32_t dim, const uint32_t* d_slot, const float* d_weights, void* d_out,
+                          uint64_t out_stride);
+
+/* Gradients of mvr_group_rows_device for dout (n * columns rows):
+ *   dx[i] = sum over c of weights[i, c] * dout[slot[i, c]]
+ *   dweights[i, c] = dot(x[i], dout[slot[i, c]])
+ * dweights may be NULL, and x with it. */
+int mvr_group_rows_grad_device(mvr_ctx* ctx, const void* d_dout, int dtype, uint64_t dout_stride, uint64_t n,
+                               uint32_t columns, uint32_t dim, const uint32_t* d_slot, const float* d_weights,
+                               const void* d_x, uint64_t x_stride, void* d_dx, uint64_t dx_stride,
+                               float* d_dweights);
+
+/* Sorted rows back to their tokens, weighted and summed:
+ *   out[i] = sum over c of weights[i, c] * xs[slot[i, c]]
+ * in the order of c; a token none of whose ids names a row gets zeros. */
+int mvr_ungroup_rows_device(mvr_ctx* ctx, const void* d_xs, int dtype, uint64_t xs_stride, uint64_t n,
+                            uint32_t columns, uint32_t dim, const uint32_t* d_slot, const float* d_weights,
+                            void* d_out, uint64_t out_stride);
+
+/* Gradients of mvr_ungroup_rows_device for dout (n x dim):
+ *   dxs[slot[i, c]] = weights[i, c] * dout[i]   (rows behind the last sorted
+ *                     row are left as they are)
+ *   dweights[i, c]  = dot(dout[i], xs[slot[i, c]])
+ * dweights may be NULL, and xs with it. */
+int mvr_ungroup_rows_grad_device(mvr_ctx* ctx, const void* d_dout, int dtype, uint64_t dout_stride, uint64_t n,
+                                 uint32_t columns, uint32_t dim, const uint32_t* d_slot, const float* d_weights,
+                                 const void* d_xs, uint64_t xs_stride, void* d_dxs, uint64_t dxs_stride,
+                                 float* d_dweights);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

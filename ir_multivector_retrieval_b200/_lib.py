@@ -251,6 +251,25 @@ SIGNATURES = {
     "mvr_hnsw_free": (None, [_P]),
     "mvr_normalize_rows": (C.c_int, [_P, _P, C.c_uint64, C.c_uint32]),
     "mvr_normalize_rows_device": (C.c_int, [_P, _P, C.c_uint64, C.c_uint32]),
+    "mvr_lookup_device": (
+        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint32, C.c_uint64, _P, C.c_int, C.c_uint64, _P, C.c_float, _P,
+                  C.c_uint64]),
+    "mvr_token_plan_bytes": (C.c_int, [C.c_uint64, C.c_uint64, _U64]),
+    "mvr_token_plan_device": (C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, _P, _P, _P, _P, _P, C.c_uint64]),
+    "mvr_lookup_grad_bytes": (C.c_int, [C.c_uint64, C.c_uint32, _U64]),
+    "mvr_lookup_grad_device": (
+        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, _P, _P, _P, _P, _P, C.c_float, _P,
+                  C.c_uint64, _P, C.c_int, C.c_uint64, C.c_int, _P, _P, C.c_uint64]),
+    "mvr_group_rows_device": (
+        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_uint64]),
+    "mvr_group_rows_grad_device": (
+        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_uint64, _P,
+                  C.c_uint64, _P]),
+    "mvr_ungroup_rows_device": (
+        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_uint64]),
+    "mvr_ungroup_rows_grad_device": (
+        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_uint64, _P,
+                  C.c_uint64, _P]),
     "mvr_tac_allocate_budgets": (
         C.c_int, [_P, _P, _P, _P, C.c_uint64, C.c_uint32, C.POINTER(ClusteringParams)]),
 }
@@ -300,6 +319,8 @@ class Context:
             raise MvrError(st, f"mvr_ctx_create(device={device})")
         self.handle = h
         self.device = device
+        self.stream = 0  # the stream given to set_stream; 0: the context's own
+        self.lock = threading.Lock()  # held by calls that switch the stream for their duration
 
     def check(self, status: int, what: str = "") -> None:
         if status != 0:
@@ -308,6 +329,7 @@ class Context:
 
     def set_stream(self, stream_handle: int | None) -> None:
         self.check(self.lib.mvr_ctx_set_stream(self.handle, C.c_void_p(stream_handle or 0)))
+        self.stream = int(stream_handle or 0)
 
     def sync(self) -> None:
         self.check(self.lib.mvr_ctx_sync(self.handle))
