@@ -693,10 +693,13 @@ int mvr_normalize_rows_device(mvr_ctx* ctx, float* d_rows, uint64_t n_floats, ui
  * unknown types, strides of outputs below dim, pointers that are not aligned
  * to their element type, rows == 0, rows >= 2^31 - 1, more than 2^31 - 1 ids
  * (plan and what uses one), a workspace below the size asked for; with
- * MVR_E_DIM_MISMATCH: dim == 0.
+ * MVR_E_DIM_MISMATCH: dim == 0. dim is at most MVR_MAX_ROW_DIM.
  * ------------------------------------------------------------------------ */
 
 enum mvr_dtype { MVR_F32 = 0, MVR_BF16 = 1, MVR_F16 = 2 };
+
+/* Longest row of the token operators. */
+#define MVR_MAX_ROW_DIM 1048576u
 
 /* Slot of a pair whose id names no row. */
 #define MVR_NO_SLOT 0xFFFFFFFFu
@@ -714,7 +717,7 @@ int mvr_token_plan_bytes(uint64_t n_ids, uint64_t rows, uint64_t* bytes);
  *   offsets[v]  first sorted place of id v (rows + 1 entries); offsets[rows]
  *               is the number of ids that name a row
  *   order[p]    the id at sorted place p (ascending inside one v), n_ids
- *               entries; those at and after offsets[rows] are undefined
+ *               entries; from offsets[rows] on the ids that name no row
  *   keys[p]     the value v at sorted place p, n_ids entries; at and after
  *               offsets[rows] they are `rows`
  *   slot[i]     the sorted place of id i, MVR_NO_SLOT where it names no row;

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
+#include <type_traits>
 
 #include "../../include/mvr.h"
 #include "km_engine.h"
@@ -31,6 +33,90 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// V consecutive elements of a row as they lie in memory: 2 to 16 bytes (32
+// for f32 sums beside 8 16-bit elements), aligned to that size up to 16, so
+// each is one access or two. Rows in flight are kept in this form.
+template <class T, int V>
+struct Raw {
+  static constexpr int kBytes = (int)sizeof(T) * V;
+  static constexpr int kWords = (kBytes + 3) / 4;
+  static_assert(kBytes <= 32, "one or two accesses");
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* __restrict__ p) {
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int h = 0; h < kBytes / 16; ++h) {
+        const uint4 r = __ldg(reinterpret_cast<const uint4*>(p) + h);
+        w[h * 4] = r.x;
+        w[h * 4 + 1] = r.y;
+        w[h * 4 + 2] = r.z;
+        w[h * 4 + 3] = r.w;
+      }
+    } else if constexpr (kBytes == 8) {
+      const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = r.x;
+      w[1] = r.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+    }
+  }
+
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int h = 0; h < kBytes / 16; ++h)
+        reinterpret_cast<uint4*>(p)[h] = make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]);
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    } else {
+      *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
+    }
+  }
+
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+
+  __device__ __forceinline__ float get(int v) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[v]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      return __uint_as_float(v & 1 ? w[v / 2] & 0xFFFF0000u : w[v / 2] << 16);
+    } else {
+      return __half2float(__ushort_as_half((unsigned short)(v & 1 ? w[v / 2] >> 16 : w[v / 2] & 0xFFFFu)));
+    }
+  }
+
+  // rounds each to the element type
+  __device__ __forceinline__ void set(const float (&x)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) w[v] = __float_as_uint(x[v]);
+    } else if constexpr (V == 1) {
+      const T t = from_f32<T>(x[0]);
+      w[0] = *reinterpret_cast<const unsigned short*>(&t);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+};
 
 // The row an id names, or `rows` where it names none (negative ids are large
 // as unsigned values).
@@ -98,26 +184,279 @@ plan_finish_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict
 }
 
 // ---- lookup gradients ------------------------------------------------------
+//
+// dtable is a sum over the sorted places of each key. The places are cut into
+// tiles of one size whatever the keys are, so a key with a seventh of all
+// tokens costs no more time than one with few: a group of L lanes sums Tg
+// consecutive places in registers, 16 bytes of the row a lane, and writes the
+// rows of the keys that begin and end among them. What a key has in a group
+// it does not begin or end in goes through shared memory to the block's other
+// groups, and what it has in a block it does not begin or end in through the
+// workspace to lookup_grad_join_kernel. Every sum's order is fixed by the
+// places, so results do not depend on which block runs first.
 
-// One warp per table row: its tokens' gradients in sorted order.
-template <class T, class O>
+// Chunks a lane holds: V elements of a row are at most 16 bytes; rows that
+// cannot be read 16 bytes at a time take several.
+template <class T, int V>
+constexpr int chunks_per_lane() {
+  return (int)sizeof(T) * V >= 16 ? 1 : (int)sizeof(T) * V >= 8 ? 2 : 4;
+}
+
+struct GradShape {
+  uint32_t n, rows, dim;
+  uint32_t lanes;     // L: lanes of a group, a power of two
+  uint32_t per_group;  // Tg: places of a group, a multiple of 8
+  uint64_t gs, ts, ds;  // row strides of grad, table, dtable
+};
+
+template <class T, class O, int V>
+struct GradArgs {
+  GradShape s;
+  const T* grad;
+  const uint32_t *offsets, *order, *keys;
+  const float* scale;
+  float alpha;
+  const T* table;
+  O* dtable;
+  int accumulate;
+  float* dscale;
+  float* part;  // [tile][2][dim]: 0 the end of a key that began before the tile, 1 what goes on behind it
+};
+
+template <class O, int V>
+__device__ __forceinline__ void put_sum(O* p, const float (&sum)[V], int accumulate) {
+  Raw<O, V> r;
+  if (accumulate) {
+    float x[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = to_f32(p[v]) + sum[v];
+    r.set(x);
+  } else {
+    r.set(sum);
+  }
+  r.store(p);
+}
+
+template <class T, class O, int V, bool DSCALE>
 __global__ void __launch_bounds__(256)
-lookup_grad_kernel(const T* __restrict__ grad, uint64_t gs, uint32_t n, uint32_t rows, uint32_t dim,
-                   const uint32_t* __restrict__ offsets, const uint32_t* __restrict__ order,
-                   const float* __restrict__ scale, float alpha, O* __restrict__ dtable, uint64_t ds, int accumulate) {
-  const int lane = threadIdx.x & 31;
-  for (uint64_t v = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); v < rows; v += (uint64_t)gridDim.x * 8) {
-    const uint32_t lo = min(offsets[v], n), hi = min(offsets[v + 1], n);
-    if (accumulate && lo >= hi) continue;
-    for (uint32_t d = lane; d < dim; d += 32) {
-      float acc = 0.f;
-      for (uint32_t p = lo; p < hi; ++p) {
-        const uint32_t i = order[p];
-        if (i < n) acc += (scale ? alpha * scale[i] : alpha) * to_f32(grad[i * gs + d]);
+lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
+  constexpr int NCH = chunks_per_lane<T, V>();
+  constexpr int U = DSCALE ? 4 : 8;  // rows in flight a lane
+  __shared__ float s_head[256 * NCH * V], s_tail[256 * NCH * V];
+  __shared__ uint8_t s_hkind[256], s_has_tail[256];  // head: 0 none, 1 ends here, 2 goes on
+  __shared__ uint32_t s_hkey[256], s_tkey[256];
+  const GradShape& S = A.s;
+  const uint32_t L = S.lanes, G = 256 / L;
+  const uint32_t g = threadIdx.x / L, l = threadIdx.x & (L - 1);
+  const uint32_t valid = min(A.offsets[S.rows], S.n);
+  const uint32_t tile = G * S.per_group;
+  const uint64_t tile0 = (uint64_t)blockIdx.x * tile;
+  if constexpr (DSCALE) {  // the tokens behind the last place name no row
+    const uint64_t end = min((uint64_t)S.n, tile0 + tile);
+    for (uint64_t p = max((uint64_t)valid, tile0) + threadIdx.x; p < end; p += 256)
+      if (A.order[p] < S.n) A.dscale[A.order[p]] = 0.f;
+  }
+  if (tile0 >= valid) return;
+  const uint32_t a = (uint32_t)min((uint64_t)valid, tile0 + (uint64_t)g * S.per_group);
+  const uint32_t b = (uint32_t)min((uint64_t)valid, tile0 + (uint64_t)(g + 1) * S.per_group);
+  uint32_t col[NCH];
+  bool on[NCH];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    col[k] = ((blockIdx.y * NCH + k) * L + l) * V;
+    on[k] = col[k] < S.dim;
+  }
+  float acc[NCH][V];
+  auto clear = [&]() {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[k][v] = 0.f;
+  };
+  clear();
+
+  bool started = a < b && (a == 0 || A.keys[a - 1] != A.keys[a]);
+  uint32_t cur = a < b ? A.keys[a] : S.rows;
+  uint32_t hkind = 0;
+  auto stage = [&](float* where) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) where[((g * NCH + k) * V + v) * L + l] = acc[k][v];
+  };
+  auto write = [&](uint32_t key) {
+    if (key < S.rows)
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+        if (on[k]) put_sum(A.dtable + (uint64_t)key * S.ds + col[k], acc[k], A.accumulate);
+  };
+
+  const uint32_t steps = (S.per_group + U - 1) / U;  // the same for all lanes: shuffles inside
+  for (uint32_t step = 0; step < steps; ++step) {
+    const uint32_t p0 = a + step * U;
+    if (__all_sync(0xffffffffu, p0 >= b)) break;
+    uint32_t key[U], tok[U];
+    float f[U];
+    Raw<T, V> row[U][NCH], trow[DSCALE ? U : 1][NCH];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = p0 + u < b;
+      key[u] = in ? A.keys[p0 + u] : S.rows;
+      tok[u] = in ? A.order[p0 + u] : S.n;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = tok[u] < S.n && key[u] < S.rows;
+      f[u] = in ? (A.scale ? A.alpha * A.scale[tok[u]] : A.alpha) : 0.f;
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        row[u][k].zero();
+        if (in && on[k]) row[u][k].load(A.grad + tok[u] * S.gs + col[k]);
+        if constexpr (DSCALE) {
+          trow[u][k].zero();
+          if (in && on[k]) trow[u][k].load(A.table + key[u] * S.ts + col[k]);
+        }
       }
-      O* o = dtable + v * ds + d;
+    }
+    if constexpr (DSCALE) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float dot = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+          for (int v = 0; v < V; ++v) dot = fmaf(row[u][k].get(v), trow[u][k].get(v), dot);
+        for (uint32_t o = L >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (l == 0 && tok[u] < S.n) A.dscale[tok[u]] = A.alpha * dot;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p0 + u < b) {
+        if (key[u] != cur) {
+          if (started) {
+            write(cur);
+          } else {
+            stage(s_head);
+            hkind = 1;
+            if (l == 0) s_hkey[g] = cur;
+          }
+          started = true;
+          cur = key[u];
+          clear();
+        }
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[k][v] = fmaf(f[u], row[u][k].get(v), acc[k][v]);
+      }
+    }
+  }
+  bool has_tail = false;
+  if (a < b) {
+    const bool ends = b == valid || A.keys[b] != cur;
+    if (started && ends) {
+      write(cur);
+    } else if (!started) {
+      stage(s_head);
+      hkind = ends ? 1 : 2;
+      if (l == 0) s_hkey[g] = cur;
+    } else {
+      stage(s_tail);
+      has_tail = true;
+      if (l == 0) s_tkey[g] = cur;
+    }
+  }
+  if (l == 0) {
+    s_hkind[g] = (uint8_t)hkind;
+    s_has_tail[g] = has_tail;
+  }
+  __syncthreads();
+
+  // a group that began a key which goes on adds what the next groups have of
+  // it; the first group does the same for a key that began in an earlier block
+  const bool from_before = g == 0 && s_hkind[0] != 0;
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+    if (turn == 0 ? !from_before : !s_has_tail[g]) continue;
+    const uint32_t key = turn == 0 ? s_hkey[0] : s_tkey[g];
+    const float* first = turn == 0 ? s_head : s_tail;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[k][v] = first[((g * NCH + k) * V + v) * L + l];
+    bool open = turn == 1 || s_hkind[0] == 2;
+    for (uint32_t q = g + 1; open && q < G && s_hkind[q] != 0; ++q) {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[k][v] += s_head[((q * NCH + k) * V + v) * L + l];
+      open = s_hkind[q] == 2;
+    }
+    if (turn == 1 && !open) {
+      write(key);
+    } else {
+      float* out = A.part + ((uint64_t)blockIdx.x * 2 + (open ? 1 : 0)) * S.dim;
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+        if (on[k])
+#pragma unroll
+          for (int v = 0; v < V; ++v) out[col[k] + v] = acc[k][v];
+    }
+  }
+}
+
+// Rows without a token become zeros (blocks from `joins` on), and block t <
+// joins sums the key that crosses the border of tiles t and t + 1 and has
+// crossed no earlier one: what it left behind the tiles, in their order, then
+// its end.
+template <class O, int V>
+__global__ void __launch_bounds__(256)
+lookup_grad_join_kernel(GradShape S, uint32_t tile, uint32_t joins, const uint32_t* __restrict__ offsets,
+                        const uint32_t* __restrict__ keys, const float* __restrict__ part, O* __restrict__ dtable,
+                        int accumulate) {
+  if (blockIdx.x >= joins) {
+    if (accumulate) return;
+    const uint32_t chunks = S.dim / V;
+    const uint64_t total = (uint64_t)S.rows * chunks;
+    for (uint64_t e = (uint64_t)(blockIdx.x - joins) * 256 + threadIdx.x; e < total;
+         e += (uint64_t)(gridDim.x - joins) * 256) {
+      const uint32_t v = (uint32_t)(e / chunks), c = (uint32_t)(e - (uint64_t)v * chunks);
+      if (offsets[v] == offsets[v + 1]) {
+        Raw<O, V> z;
+        z.zero();
+        z.store(dtable + v * S.ds + c * V);
+      }
+    }
+    return;
+  }
+  const uint32_t valid = min(offsets[S.rows], S.n);
+  const uint64_t border = (uint64_t)(blockIdx.x + 1) * tile;
+  if (border >= valid) return;
+  const uint32_t key = keys[border];
+  if (key >= S.rows || keys[border - 1] != key) return;
+  const uint32_t first = offsets[key] / tile, last = (min(offsets[key + 1], valid) - 1) / tile;
+  if (first != blockIdx.x) return;
+  __shared__ float s_sum[256];
+  // 32 columns at a time, 8 warps over the tiles
+  const uint32_t w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  for (uint32_t c0 = 0; c0 < S.dim; c0 += 32) {
+    const uint32_t c = c0 + l;
+    float acc = 0.f;
+    if (c < S.dim) {
+#pragma unroll 8
+      for (uint32_t t = first + w; t < last; t += 8) acc += part[((uint64_t)t * 2 + 1) * S.dim + c];
+    }
+    s_sum[threadIdx.x] = acc;
+    __syncthreads();
+    if (w == 0 && c < S.dim) {
+#pragma unroll
+      for (int q = 1; q < 8; ++q) acc += s_sum[q * 32 + l];
+      acc += part[(uint64_t)last * 2 * S.dim + c];
+      O* o = dtable + (uint64_t)key * S.ds + c;
       *o = from_f32<O>(accumulate ? to_f32(*o) + acc : acc);
     }
+    __syncthreads();
   }
 }
 
@@ -210,6 +549,37 @@ unsigned warp_grid(Ctx* c, uint64_t n) {
   return (unsigned)std::min<uint64_t>((n + 7) / 8, (uint64_t)c->sm_count * 32);
 }
 
+// Largest number of elements, at most 16 bytes, by which the row length, the
+// strides and the addresses can all be divided: how wide a lane reads.
+struct Rows {
+  const void* p;
+  uint64_t stride;
+};
+int vec_of(int dtype, uint32_t dim, std::initializer_list<Rows> all) {
+  const uint64_t e = elem_size(dtype);
+  uint64_t bits = 16 / e | dim;
+  for (const Rows& r : all)
+    if (r.p) bits |= r.stride | reinterpret_cast<uintptr_t>(r.p) / e;
+  return (int)(bits & (~bits + 1));
+}
+
+uint32_t pow2_ceil(uint32_t v) {
+  uint32_t p = 1;
+  while (p < v) p <<= 1;
+  return p;
+}
+
+// Calls f with the width as a compile-time number.
+template <class T, class F>
+int by_vec(int v, F&& f) {
+  if constexpr (sizeof(T) == 2) {
+    if (v >= 8) return f(std::integral_constant<int, 8>());
+  }
+  if (v >= 4) return f(std::integral_constant<int, 4>());
+  if (v >= 2) return f(std::integral_constant<int, 2>());
+  return f(std::integral_constant<int, 1>());
+}
+
 // Calls f with a null pointer of the element type.
 template <class F>
 int by_type(int dtype, F&& f) {
@@ -234,6 +604,7 @@ int check_rows(Ctx* c, const char* what, const void* p, int dtype, uint64_t n, u
                bool output) {
   if (!known(dtype)) return bad(c, "unknown element type");
   if (dim == 0) return fail(c, MVR_E_DIM_MISMATCH, "dim == 0");
+  if (dim > MVR_MAX_ROW_DIM) return bad(c, "dim above MVR_MAX_ROW_DIM");
   if (n && !p) return fail(c, MVR_E_INVALID_ARGUMENT, std::string("null pointer: ") + what);
   if (!aligned(p, elem_size(dtype)))
     return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + " is not aligned to its element type");
@@ -281,6 +652,46 @@ struct PlanSpace {
     total = off;
   }
 };
+
+// Smallest block of places, whatever the row length: the workspace is sized
+// for it. 8 places a group, 8 groups of 32 lanes at least.
+constexpr uint32_t kMinTile = 64;
+
+template <class T, class O, int V>
+int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
+  GradShape& S = A.s;
+  cudaStream_t st = c->stream;
+  constexpr uint32_t NCH = chunks_per_lane<T, V>();
+  const uint32_t chunks = S.dim / V;
+  S.lanes = std::min(32u, pow2_ceil((chunks + NCH - 1) / NCH));
+  const uint32_t slabs = (chunks + S.lanes * NCH - 1) / (S.lanes * NCH);
+  const uint32_t groups = 256 / S.lanes;
+  // Long groups leave fewer sums to join, short ones more blocks: the longest
+  // of 8 to 64 places that still gives every SM eight blocks.
+  S.per_group = 64;
+  while (S.per_group > 8 &&
+         (uint64_t)slabs * ((S.n + (uint64_t)groups * S.per_group - 1) / ((uint64_t)groups * S.per_group)) <
+             8ull * c->sm_count)
+    S.per_group >>= 1;
+  const uint32_t tile = groups * S.per_group;
+  const uint32_t tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
+  if (tiles) {
+    if (A.dscale && slabs == 1)
+      lookup_grad_tile_kernel<T, O, V, true><<<dim3(tiles, slabs), 256, 0, st>>>(A);
+    else
+      lookup_grad_tile_kernel<T, O, V, false><<<dim3(tiles, slabs), 256, 0, st>>>(A);
+    if (A.dscale && slabs > 1)  // a row's parts lie in several blocks
+      lookup_dscale_kernel<T><<<warp_grid(c, S.n), 256, 0, st>>>(A.grad, S.gs, S.n, S.rows, S.dim, A.keys, slot,
+                                                                A.alpha, A.table, S.ts, A.dscale);
+  }
+  const uint32_t joins = tiles ? tiles - 1 : 0;
+  const uint64_t fill = A.accumulate ? 0 : std::min<uint64_t>(((uint64_t)S.rows * chunks + 255) / 256, 8ull * c->sm_count);
+  if (joins + fill)
+    lookup_grad_join_kernel<O, V><<<(unsigned)(joins + fill), 256, 0, st>>>(S, tile, joins, A.offsets, A.keys, A.part,
+                                                                           A.dtable, A.accumulate);
+  MVR_CUDA(c, cudaGetLastError());
+  return MVR_OK;
+}
 
 int spread(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t columns, uint32_t dim,
            const uint32_t* slot, const float* w, void* dst, uint64_t ds, const void* other, uint64_t os, float* dw) {
@@ -383,7 +794,7 @@ int mvr_token_plan_device(mvr_ctx* h, const void* d_ids, int id_bytes, uint64_t 
 
 int mvr_lookup_grad_bytes(uint64_t n_ids, uint32_t dim, uint64_t* bytes) {
   if (!bytes || n_ids > mvr::kMaxIds || dim == 0) return MVR_E_INVALID_ARGUMENT;
-  *bytes = 0;
+  *bytes = (n_ids + mvr::kMinTile - 1) / mvr::kMinTile * 2 * dim * sizeof(float);
   return MVR_OK;
 }
 
@@ -411,24 +822,35 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
   MVR_TRY(mvr::check_workspace(c, d_workspace, workspace_bytes, need));
   mvr::DeviceScope dev_scope(c);
   MVR_TRY(dev_scope.status);
-  cudaStream_t st = c->stream;
   const uint32_t n = (uint32_t)n_ids, v = (uint32_t)rows;
   return mvr::by_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (dtable_dtype == MVR_F32)
-      mvr::lookup_grad_kernel<T, float><<<mvr::warp_grid(c, v), 256, 0, st>>>(
-          (const T*)d_grad, grad_stride, n, v, dim, d_offsets, d_order, d_scale, alpha, (float*)d_dtable,
-          dtable_stride, accumulate);
-    else
-      mvr::lookup_grad_kernel<T, T><<<mvr::warp_grid(c, v), 256, 0, st>>>((const T*)d_grad, grad_stride, n, v, dim,
-                                                                          d_offsets, d_order, d_scale, alpha,
-                                                                          (T*)d_dtable, dtable_stride, accumulate);
-    if (d_dscale && n)
-      mvr::lookup_dscale_kernel<T><<<mvr::warp_grid(c, n), 256, 0, st>>>((const T*)d_grad, grad_stride, n, v, dim,
-                                                                         d_keys, d_slot, alpha, (const T*)d_table,
-                                                                         table_stride, d_dscale);
-    MVR_CUDA(c, cudaGetLastError());
-    return (int)MVR_OK;
+    auto run = [&](auto* o) {
+      using O = std::remove_pointer_t<decltype(o)>;
+      int w = mvr::vec_of(dtype, dim, {{d_grad, grad_stride}, {d_dscale ? d_table : nullptr, table_stride}});
+      // 8 f32 sums are two 16-byte accesses, so 16-byte alignment serves them too
+      const int wo = mvr::vec_of(dtable_dtype, dim, {{d_dtable, dtable_stride}});
+      w = std::min(w, sizeof(O) > sizeof(T) && wo == 4 ? 8 : wo);
+      return mvr::by_vec<T>(w, [&](auto vec) {
+        constexpr int V = decltype(vec)::value;
+        mvr::GradArgs<T, O, V> A;
+        A.s = {n, v, dim, 0, 0, grad_stride, table_stride, dtable_stride};
+        A.grad = (const T*)d_grad;
+        A.offsets = d_offsets;
+        A.order = d_order;
+        A.keys = d_keys;
+        A.scale = d_scale;
+        A.alpha = alpha;
+        A.table = (const T*)d_table;
+        A.dtable = (O*)d_dtable;
+        A.accumulate = accumulate;
+        A.dscale = d_dscale;
+        A.part = (float*)d_workspace;
+        return mvr::lookup_grad_run(c, A, d_slot);
+      });
+    };
+    if (dtable_dtype == MVR_F32) return run(static_cast<float*>(nullptr));
+    return run(t);
   });
 }
 

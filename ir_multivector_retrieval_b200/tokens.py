@@ -176,7 +176,7 @@ class Plan:
     ``keys[p]`` its value, ``offsets`` (rows + 1) the first place of each
     value; ``slot`` has the ids' shape and holds each one's place, -1 where it
     names no row. ``offsets[rows]`` is the number of ids that name a row;
-    ``order`` is undefined from there on and ``keys`` is ``rows``."""
+    from there on ``order`` lists those that name none and ``keys`` is ``rows``."""
 
     rows: int
     offsets: object
