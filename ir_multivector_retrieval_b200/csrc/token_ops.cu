@@ -20,6 +20,7 @@ namespace {
 
 constexpr uint32_t kNoSlot = MVR_NO_SLOT;
 constexpr uint64_t kMaxIds = 0x7FFFFFFFull;   // pairs of a plan: places fit 31 bits
+constexpr uint64_t kMaxElems = 1ull << 38;
 constexpr uint64_t kMaxRows = 0x7FFFFFFEull;  // rows + 1 offsets, and `rows` itself is the key of no row
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -126,26 +127,93 @@ __device__ __forceinline__ uint32_t row_of(const void* ids, int id_bytes, uint64
   return v < rows ? (uint32_t)v : rows;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Sum of x over the lanes of a group (L a power of two up to 256), in lane 0.
+// s: one value a warp; every thread of the block calls it.
+__device__ __forceinline__ float group_sum(float x, uint32_t L, float* s) {
+  for (uint32_t o = min(L, 32u) >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (L > 32) {
+    const uint32_t warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) s[warp] = x;
+    __syncthreads();
+    if ((threadIdx.x & (L - 1)) == 0)
+      for (uint32_t q = 1; q < L / 32; ++q) x += s[warp + q];
+    __syncthreads();
+  }
+  return x;
 }
 
 // ---- lookup ----------------------------------------------------------------
+//
+// Bound by memory: the table's rows that are named are read, every output row
+// is written. One thread per V elements, numbered through the whole output,
+// so that a warp writes one run of memory whatever the row length; four of
+// them a thread, the block's stride apart, when there is work for all SMs.
 
-// One warp per row.
-template <class T>
+// Where element `e` of the outputs lies: row and chunk of a row. `shift` is
+// log2(chunks) or -1.
+struct Flat {
+  uint64_t total;  // rows x chunks
+  uint32_t chunks;
+  int shift;
+};
+
+template <int UR>
+struct FlatBlock {
+  uint64_t first, row0;
+  uint32_t rem0;
+  const Flat F;
+  __device__ __forceinline__ explicit FlatBlock(const Flat& f) : F(f) {
+    first = (uint64_t)blockIdx.x * (256 * UR);
+    row0 = F.shift >= 0 ? first >> F.shift : first / F.chunks;
+    rem0 = (uint32_t)(first - row0 * F.chunks);
+  }
+  // false behind the end
+  __device__ __forceinline__ bool at(int j, uint64_t* row, uint32_t* chunk) const {
+    const uint32_t local = j * 256 + threadIdx.x;
+    if (first + local >= F.total) return false;
+    const uint32_t x = rem0 + local;
+    const uint32_t q = F.shift >= 0 ? x >> F.shift : x / F.chunks;
+    *row = row0 + q;
+    *chunk = x - q * F.chunks;
+    return true;
+  }
+};
+
+template <class T, int V, int UR>
 __global__ void __launch_bounds__(256)
-lookup_kernel(const T* __restrict__ table, uint32_t rows, uint32_t dim, uint64_t ts, const void* __restrict__ ids,
-              int id_bytes, uint64_t n, const float* __restrict__ scale, float alpha, T* __restrict__ out,
-              uint64_t os) {
-  const int lane = threadIdx.x & 31;
-  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (uint64_t)gridDim.x * 8) {
-    const uint32_t r = row_of(ids, id_bytes, i, rows);
-    const float f = scale ? alpha * scale[i] : alpha;
-    for (uint32_t d = lane; d < dim; d += 32)
-      out[i * os + d] = r < rows ? from_f32<T>(f * to_f32(table[r * ts + d])) : from_f32<T>(0.f);
+lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, const void* __restrict__ ids,
+              int id_bytes, const float* __restrict__ scale, float alpha, T* __restrict__ out, uint64_t os) {
+  const FlatBlock<UR> B(F);
+  uint64_t i[UR];
+  uint32_t c[UR], r[UR];
+  float f[UR];
+  Raw<T, V> x[UR];
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    r[j] = rows;
+    f[j] = alpha;
+    if (B.at(j, &i[j], &c[j])) {
+      r[j] = row_of(ids, id_bytes, i[j], rows);
+      if (scale) f[j] = alpha * scale[i[j]];
+    } else {
+      i[j] = ~0ull;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    x[j].zero();
+    if (r[j] < rows) x[j].load(table + r[j] * ts + (uint64_t)c[j] * V);
+  }
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    if (i[j] == ~0ull) continue;
+    if (r[j] < rows) {
+      float y[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) y[v] = f[j] * x[j].get(v);
+      x[j].set(y);
+    }
+    x[j].store(out + i[j] * os + (uint64_t)c[j] * V);
   }
 }
 
@@ -460,82 +528,226 @@ lookup_grad_join_kernel(GradShape S, uint32_t tile, uint32_t joins, const uint32
   }
 }
 
-// One warp per token; its table row is the key at its place.
-template <class T>
+// dscale where a row's parts lie in several blocks of the sums: a group of L
+// lanes per token, its table row is the key at its place.
+template <class T, int V>
 __global__ void __launch_bounds__(256)
-lookup_dscale_kernel(const T* __restrict__ grad, uint64_t gs, uint32_t n, uint32_t rows, uint32_t dim,
+lookup_dscale_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ grad, uint64_t gs, uint32_t n, uint32_t rows,
                      const uint32_t* __restrict__ keys, const uint32_t* __restrict__ slot, float alpha,
                      const T* __restrict__ table, uint64_t ts, float* __restrict__ dscale) {
-  const int lane = threadIdx.x & 31;
-  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (uint64_t)gridDim.x * 8) {
-    const uint32_t p = slot[i], r = p < n ? keys[p] : rows;
-    float acc = 0.f;
-    if (r < rows)
-      for (uint32_t d = lane; d < dim; d += 32) acc = fmaf(to_f32(grad[i * gs + d]), to_f32(table[r * ts + d]), acc);
-    acc = warp_sum(acc);
-    if (lane == 0) dscale[i] = alpha * acc;
+  constexpr int U = 4;
+  __shared__ float s_sum[8];
+  const uint32_t l = threadIdx.x & (L - 1);
+  const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const uint32_t p = i < n ? slot[i] : kNoSlot, r = p < n ? keys[p] : rows;
+  float dot = 0.f;
+  if (r < rows) {
+    const T* a = grad + i * gs;
+    const T* b = table + r * ts;
+    for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
+      Raw<T, V> x[U], o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u].zero();
+        o[u].zero();
+        const uint32_t c = c0 + u * L;
+        if (c < chunks) {
+          x[u].load(a + (uint64_t)c * V);
+          o[u].load(b + (uint64_t)c * V);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) dot = fmaf(x[u].get(v), o[u].get(v), dot);
+    }
   }
+  dot = group_sum(dot, L, s_sum);
+  if (l == 0 && i < n) dscale[i] = alpha * dot;
 }
 
 // ---- rows into sorted order and back ---------------------------------------
+//
+// Bound by memory as well: with C choices a token, spreading reads a row and
+// writes C, collecting reads C and writes one. Without the weights' gradient
+// the work is cut as for the lookup. With it a group of lanes has a row, for
+// the dot products.
 
-// spread: one warp per token, dst[slot] = w * src[token]; with dw also the
-// dot of src[token] and other[slot].
-template <class T>
+// dst[slot[i, c]] = w[i, c] * src[i]: a token's row is read once.
+template <class T, int V, int UR>
 __global__ void __launch_bounds__(256)
-spread_kernel(const T* __restrict__ src, uint64_t ss, uint64_t n, uint32_t columns, uint32_t dim,
-              const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds,
-              const T* __restrict__ other, uint64_t other_s, float* __restrict__ dw) {
-  const int lane = threadIdx.x & 31;
-  const uint64_t pairs = n * columns;
-  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (uint64_t)gridDim.x * 8) {
-    for (uint32_t c = 0; c < columns; ++c) {
-      const uint32_t p = slot[i * columns + c];
-      const bool ok = p < pairs;
-      const float f = w ? w[i * columns + c] : 1.f;
-      float acc = 0.f;
-      if (ok)
-        for (uint32_t d = lane; d < dim; d += 32) {
-          const float x = to_f32(src[i * ss + d]);
-          dst[p * ds + d] = from_f32<T>(f * x);
-          if (dw) acc = fmaf(x, to_f32(other[p * other_s + d]), acc);
-        }
-      if (dw) {
-        acc = warp_sum(acc);
-        if (lane == 0) dw[i * columns + c] = acc;
+spread_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
+              const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds) {
+  const FlatBlock<UR> B(F);
+  uint64_t i[UR];
+  uint32_t c[UR];
+  Raw<T, V> x[UR];
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    if (B.at(j, &i[j], &c[j]))
+      x[j].load(src + i[j] * ss + (uint64_t)c[j] * V);
+    else
+      i[j] = ~0ull;
+  }
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    if (i[j] == ~0ull) continue;
+    for (uint32_t k = 0; k < columns; ++k) {
+      const uint32_t p = slot[i[j] * columns + k];
+      if (p >= pairs) continue;
+      Raw<T, V> r = x[j];
+      if (w) {
+        const float f = w[i[j] * columns + k];
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = f * x[j].get(v);
+        r.set(y);
       }
+      r.store(dst + p * ds + (uint64_t)c[j] * V);
     }
   }
 }
 
-// collect: one warp per token, dst[token] = sum_c w * src[slot]; with dw also
-// the dot of other[token] and src[slot].
-template <class T>
+// dst[i] = sum_c w[i, c] * src[slot[i, c]]: KU choices' rows in flight.
+template <class T, int V, int KU>
 __global__ void __launch_bounds__(256)
-collect_kernel(const T* __restrict__ src, uint64_t ss, uint64_t n, uint32_t columns, uint32_t dim,
-               const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds,
-               const T* __restrict__ other, uint64_t other_s, float* __restrict__ dw) {
-  const int lane = threadIdx.x & 31;
-  const uint64_t pairs = n * columns;
-  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += (uint64_t)gridDim.x * 8) {
-    for (uint32_t d = lane; d < dim; d += 32) {
-      float acc = 0.f;
-      for (uint32_t c = 0; c < columns; ++c) {
-        const uint32_t p = slot[i * columns + c];
-        if (p < pairs) acc = fmaf(w ? w[i * columns + c] : 1.f, to_f32(src[p * ss + d]), acc);
+collect_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
+               const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds) {
+  const FlatBlock<1> B(F);
+  uint64_t i;
+  uint32_t c;
+  if (!B.at(0, &i, &c)) return;
+  float acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  for (uint32_t k0 = 0; k0 < columns; k0 += KU) {
+    Raw<T, V> x[KU];
+    float f[KU];
+    uint32_t p[KU];
+#pragma unroll
+    for (int k = 0; k < KU; ++k) p[k] = k0 + k < columns ? slot[i * columns + k0 + k] : kNoSlot;
+#pragma unroll
+    for (int k = 0; k < KU; ++k) {
+      if (p[k] < pairs) {
+        x[k].load(src + p[k] * ss + (uint64_t)c * V);
+        f[k] = w ? w[i * columns + k0 + k] : 1.f;
+      } else {
+        x[k].zero();
+        f[k] = 0.f;
       }
-      dst[i * ds + d] = from_f32<T>(acc);
     }
-    if (dw)
-      for (uint32_t c = 0; c < columns; ++c) {
-        const uint32_t p = slot[i * columns + c];
-        float acc = 0.f;
-        if (p < pairs)
-          for (uint32_t d = lane; d < dim; d += 32)
-            acc = fmaf(to_f32(other[i * other_s + d]), to_f32(src[p * ss + d]), acc);
-        acc = warp_sum(acc);
-        if (lane == 0) dw[i * columns + c] = acc;
+#pragma unroll
+    for (int k = 0; k < KU; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(f[k], x[k].get(v), acc[v]);
+  }
+  Raw<T, V> r;
+  r.set(acc);
+  r.store(dst + i * ds + (uint64_t)c * V);
+}
+
+// The pair's two rows in one pass: dst[slot] = w * src[token], dw = <src[token],
+// other[slot]>. A group of lanes has a pair, so a token's row is read once
+// from memory and again from the caches for its other choices.
+template <class T, int V, bool DST>
+__global__ void __launch_bounds__(256)
+spread_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint64_t ss, uint32_t columns,
+                  uint64_t pairs, const uint32_t* __restrict__ slot, const float* __restrict__ w,
+                  T* __restrict__ dst, uint64_t ds, const T* __restrict__ other, uint64_t other_s,
+                  float* __restrict__ dw) {
+  constexpr int U = 4;
+  __shared__ float s_sum[8];
+  const uint32_t l = threadIdx.x & (L - 1);
+  const uint64_t pair = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const uint32_t p = pair < pairs ? slot[pair] : kNoSlot;
+  float dot = 0.f;
+  if (p < pairs) {
+    const T* a = src + pair / columns * ss;
+    const T* b = other + p * other_s;
+    const float f = w ? w[pair] : 1.f;
+    for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
+      Raw<T, V> x[U], o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u].zero();
+        o[u].zero();
+        const uint32_t c = c0 + u * L;
+        if (c < chunks) {
+          x[u].load(a + (uint64_t)c * V);
+          o[u].load(b + (uint64_t)c * V);
+        }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          dot = fmaf(x[u].get(v), o[u].get(v), dot);
+          y[v] = f * x[u].get(v);
+        }
+        if constexpr (DST) {
+          const uint32_t c = c0 + u * L;
+          if (c < chunks) {
+            if (w) x[u].set(y);
+            x[u].store(dst + p * ds + (uint64_t)c * V);
+          }
+        }
+      }
+    }
+  }
+  dot = group_sum(dot, L, s_sum);
+  if (l == 0 && pair < pairs) dw[pair] = dot;
+}
+
+// dst[i] = sum_c w * src[slot] and dw = <other[i], src[slot]> in one pass, for
+// at most KU choices: a group of lanes has a token.
+template <class T, int V, int KU>
+__global__ void __launch_bounds__(256)
+collect_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint64_t ss, uint64_t n, uint32_t columns,
+                   const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds,
+                   const T* __restrict__ other, uint64_t other_s, float* __restrict__ dw) {
+  __shared__ float s_sum[8];
+  const uint64_t pairs = n * columns;
+  const uint32_t l = threadIdx.x & (L - 1);
+  const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  uint32_t p[KU];
+  float f[KU], dot[KU];
+#pragma unroll
+  for (int k = 0; k < KU; ++k) {
+    const bool in = i < n && (uint32_t)k < columns;
+    p[k] = in ? slot[i * columns + k] : kNoSlot;
+    f[k] = p[k] < pairs ? (w ? w[i * columns + k] : 1.f) : 0.f;
+    dot[k] = 0.f;
+  }
+  if (i < n)
+    for (uint32_t c = l; c < chunks; c += L) {
+      Raw<T, V> o, x[KU];
+      o.load(other + i * other_s + (uint64_t)c * V);
+      float acc[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KU; ++k) {
+        x[k].zero();
+        if (p[k] < pairs) x[k].load(src + p[k] * ss + (uint64_t)c * V);
+      }
+#pragma unroll
+      for (int k = 0; k < KU; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float xv = x[k].get(v);
+          acc[v] = fmaf(f[k], xv, acc[v]);
+          dot[k] = fmaf(o.get(v), xv, dot[k]);
+        }
+      o.set(acc);
+      o.store(dst + i * ds + (uint64_t)c * V);
+    }
+#pragma unroll
+  for (int k = 0; k < KU; ++k) {
+    if ((uint32_t)k >= columns) break;  // the same for the whole grid
+    const float d = group_sum(dot[k], L, s_sum);
+    // a choice that names no row met only zeros, but zero times an infinity is none
+    if (l == 0 && i < n) dw[i * columns + k] = p[k] < pairs ? d : 0.f;
   }
 }
 
@@ -545,9 +757,6 @@ size_t elem_size(int dtype) { return dtype == MVR_F32 ? 4 : 2; }
 bool known(int dtype) { return dtype == MVR_F32 || dtype == MVR_BF16 || dtype == MVR_F16; }
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 uint64_t up256(uint64_t v) { return (v + 255) & ~(uint64_t)255; }
-unsigned warp_grid(Ctx* c, uint64_t n) {
-  return (unsigned)std::min<uint64_t>((n + 7) / 8, (uint64_t)c->sm_count * 32);
-}
 
 // Largest number of elements, at most 16 bytes, by which the row length, the
 // strides and the addresses can all be divided: how wide a lane reads.
@@ -567,6 +776,30 @@ uint32_t pow2_ceil(uint32_t v) {
   uint32_t p = 1;
   while (p < v) p <<= 1;
   return p;
+}
+
+Flat flat_of(uint64_t n, uint32_t chunks) {
+  int shift = -1;
+  if ((chunks & (chunks - 1)) == 0)
+    for (shift = 0; (1u << shift) < chunks;) ++shift;
+  return {n * chunks, chunks, shift};
+}
+
+// Four elements a thread when that still fills every SM with threads.
+bool many(Ctx* c, const Flat& F) { return F.total >= 4ull * 2048 * c->sm_count; }
+
+// Lanes of a row for the dot products: one chunk a lane when there are few
+// rows; as many as four a lane (fewer lanes to sum over) while every SM keeps
+// 1024 threads.
+uint32_t lanes_of(Ctx* c, uint64_t n, uint32_t chunks) {
+  uint32_t L = std::min(256u, pow2_ceil(chunks));
+  while (L > 1 && chunks < 4 * L && n * (L / 2) >= 1024ull * c->sm_count) L /= 2;
+  return L;
+}
+
+// Blocks of a launch: fewer than 2^31 for all that the checks let through.
+unsigned blocks_of(uint64_t items, uint64_t per_block) {
+  return (unsigned)((items + per_block - 1) / per_block);
 }
 
 // Calls f with the width as a compile-time number.
@@ -606,6 +839,8 @@ int check_rows(Ctx* c, const char* what, const void* p, int dtype, uint64_t n, u
   if (dim == 0) return fail(c, MVR_E_DIM_MISMATCH, "dim == 0");
   if (dim > MVR_MAX_ROW_DIM) return bad(c, "dim above MVR_MAX_ROW_DIM");
   if (n && !p) return fail(c, MVR_E_INVALID_ARGUMENT, std::string("null pointer: ") + what);
+  // what one launch covers: 2^31 - 1 blocks of 256 elements
+  if (n > kMaxElems / dim) return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + ": more than 2^38 elements");
   if (!aligned(p, elem_size(dtype)))
     return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + " is not aligned to its element type");
   if (output && stride < dim) return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + ": stride below dim");
@@ -680,9 +915,11 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
       lookup_grad_tile_kernel<T, O, V, true><<<dim3(tiles, slabs), 256, 0, st>>>(A);
     else
       lookup_grad_tile_kernel<T, O, V, false><<<dim3(tiles, slabs), 256, 0, st>>>(A);
-    if (A.dscale && slabs > 1)  // a row's parts lie in several blocks
-      lookup_dscale_kernel<T><<<warp_grid(c, S.n), 256, 0, st>>>(A.grad, S.gs, S.n, S.rows, S.dim, A.keys, slot,
-                                                                A.alpha, A.table, S.ts, A.dscale);
+    if (A.dscale && slabs > 1) {  // a row's parts lie in several blocks
+      const uint32_t L = lanes_of(c, S.n, chunks);
+      lookup_dscale_kernel<T, V><<<blocks_of(S.n, 256 / L), 256, 0, st>>>(
+          L, chunks, A.grad, S.gs, S.n, S.rows, A.keys, slot, A.alpha, A.table, S.ts, A.dscale);
+    }
   }
   const uint32_t joins = tiles ? tiles - 1 : 0;
   const uint64_t fill = A.accumulate ? 0 : std::min<uint64_t>(((uint64_t)S.rows * chunks + 255) / 256, 8ull * c->sm_count);
@@ -698,26 +935,74 @@ int spread(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t
   if (n == 0) return MVR_OK;
   DeviceScope dev_scope(c);
   MVR_TRY(dev_scope.status);
+  const uint64_t pairs = n * columns;
+  const int w_ = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {dw ? other : nullptr, os}});
   return by_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    spread_kernel<T><<<warp_grid(c, n), 256, 0, c->stream>>>((const T*)src, ss, n, columns, dim, slot, w, (T*)dst, ds,
-                                                             (const T*)other, os, dw);
-    MVR_CUDA(c, cudaGetLastError());
-    return (int)MVR_OK;
+    return by_vec<T>(w_, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const uint32_t chunks = dim / V;
+      if (dw) {
+        const uint32_t L = lanes_of(c, pairs, chunks);
+        spread_dot_kernel<T, V, true><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(
+            L, chunks, (const T*)src, ss, columns, pairs, slot, w, (T*)dst, ds, (const T*)other, os, dw);
+      } else {
+        const Flat F = flat_of(n, chunks);
+        if (many(c, F))
+          spread_kernel<T, V, 4><<<blocks_of(F.total, 1024), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs,
+                                                                                  slot, w, (T*)dst, ds);
+        else
+          spread_kernel<T, V, 1><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs,
+                                                                                 slot, w, (T*)dst, ds);
+      }
+      MVR_CUDA(c, cudaGetLastError());
+      return (int)MVR_OK;
+    });
   });
 }
+
+// Choices whose dot products a lane holds at once.
+constexpr uint32_t kDotColumns = 8;
 
 int collect(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t columns, uint32_t dim,
             const uint32_t* slot, const float* w, void* dst, uint64_t ds, const void* other, uint64_t os, float* dw) {
   if (n == 0) return MVR_OK;
   DeviceScope dev_scope(c);
   MVR_TRY(dev_scope.status);
+  const uint64_t pairs = n * columns;
+  const int w_ = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {dw ? other : nullptr, os}});
   return by_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    collect_kernel<T><<<warp_grid(c, n), 256, 0, c->stream>>>((const T*)src, ss, n, columns, dim, slot, w, (T*)dst, ds,
-                                                              (const T*)other, os, dw);
-    MVR_CUDA(c, cudaGetLastError());
-    return (int)MVR_OK;
+    return by_vec<T>(w_, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const uint32_t chunks = dim / V;
+      const T *s = (const T*)src, *o = (const T*)other;
+      if (dw && columns <= kDotColumns) {
+        const uint32_t L = lanes_of(c, n, chunks);
+        const unsigned blocks = blocks_of(n, 256 / L);
+        if (columns <= 2)
+          collect_dot_kernel<T, V, 2><<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w, (T*)dst,
+                                                                     ds, o, os, dw);
+        else
+          collect_dot_kernel<T, V, kDotColumns><<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w,
+                                                                               (T*)dst, ds, o, os, dw);
+      } else {
+        const Flat F = flat_of(n, chunks);
+        if (columns <= 2)
+          collect_kernel<T, V, 2><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w,
+                                                                                  (T*)dst, ds);
+        else
+          collect_kernel<T, V, 8><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w,
+                                                                                  (T*)dst, ds);
+        if (dw) {  // the dots on their own: src once more
+          const uint32_t L = lanes_of(c, pairs, chunks);
+          spread_dot_kernel<T, V, false><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(
+              L, chunks, o, os, columns, pairs, slot, nullptr, nullptr, 0, s, ss, dw);
+        }
+      }
+      MVR_CUDA(c, cudaGetLastError());
+      return (int)MVR_OK;
+    });
   });
 }
 
@@ -740,13 +1025,23 @@ int mvr_lookup_device(mvr_ctx* h, const void* d_table, int dtype, uint64_t rows,
   if (n == 0) return MVR_OK;
   mvr::DeviceScope dev_scope(c);
   MVR_TRY(dev_scope.status);
+  const int w = mvr::vec_of(dtype, dim, {{d_table, table_stride}, {d_out, out_stride}});
   return mvr::by_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    mvr::lookup_kernel<T><<<mvr::warp_grid(c, n), 256, 0, c->stream>>>(
-        (const T*)d_table, (uint32_t)rows, dim, table_stride, d_ids, id_bytes, n, d_scale, alpha, (T*)d_out,
-        out_stride);
-    MVR_CUDA(c, cudaGetLastError());
-    return (int)MVR_OK;
+    return mvr::by_vec<T>(w, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const mvr::Flat F = mvr::flat_of(n, dim / V);
+      if (mvr::many(c, F))
+        mvr::lookup_kernel<T, V, 4><<<mvr::blocks_of(F.total, 1024), 256, 0, c->stream>>>(
+            F, (const T*)d_table, (uint32_t)rows, table_stride, d_ids, id_bytes, d_scale, alpha, (T*)d_out,
+            out_stride);
+      else
+        mvr::lookup_kernel<T, V, 1><<<mvr::blocks_of(F.total, 256), 256, 0, c->stream>>>(
+            F, (const T*)d_table, (uint32_t)rows, table_stride, d_ids, id_bytes, d_scale, alpha, (T*)d_out,
+            out_stride);
+      MVR_CUDA(c, cudaGetLastError());
+      return (int)MVR_OK;
+    });
   });
 }
 
