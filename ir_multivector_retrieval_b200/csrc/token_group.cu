@@ -1,0 +1,333 @@
+// token_group.cu — rows sorted by group (expert, centroid, token id) and back,
+// with weights applied, and their gradients. include/mvr.h states what each
+// call computes.
+#include "token_ops.cuh"
+
+namespace mvr {
+namespace tok {
+namespace {
+
+// ---- rows into sorted order and back ---------------------------------------
+//
+// Bound by memory as well: with C choices a token, spreading reads a row and
+// writes C, collecting reads C and writes one. Without the weights' gradient
+// the work is cut as for the lookup. With it a group of lanes has a row, for
+// the dot products.
+
+// dst[slot[i, c]] = w[i, c] * src[i]: a token's row is read once.
+template <class T, int V, int UR>
+__global__ void __launch_bounds__(256)
+spread_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
+              const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds) {
+  const FlatBlock<UR> B(F);
+  uint64_t i[UR];
+  uint32_t c[UR];
+  Raw<T, V> x[UR];
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    if (B.at(j, &i[j], &c[j]))
+      x[j].load(src + i[j] * ss + (uint64_t)c[j] * V);
+    else
+      i[j] = ~0ull;
+  }
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    if (i[j] == ~0ull) continue;
+    for (uint32_t k = 0; k < columns; ++k) {
+      const uint32_t p = slot[i[j] * columns + k];
+      if (p >= pairs) continue;
+      Raw<T, V> r = x[j];
+      if (w) {
+        const float f = w[i[j] * columns + k];
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = f * x[j].get(v);
+        r.set(y);
+      }
+      r.store(dst + p * ds + (uint64_t)c[j] * V);
+    }
+  }
+}
+
+// dst[i] = sum_c w[i, c] * src[slot[i, c]]: KU choices' rows in flight.
+template <class T, int V, int KU>
+__global__ void __launch_bounds__(256)
+collect_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
+               const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds) {
+  const FlatBlock<1> B(F);
+  uint64_t i;
+  uint32_t c;
+  if (!B.at(0, &i, &c)) return;
+  float acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  for (uint32_t k0 = 0; k0 < columns; k0 += KU) {
+    Raw<T, V> x[KU];
+    float f[KU];
+    uint32_t p[KU];
+#pragma unroll
+    for (int k = 0; k < KU; ++k) p[k] = k0 + k < columns ? slot[i * columns + k0 + k] : kNoSlot;
+#pragma unroll
+    for (int k = 0; k < KU; ++k) {
+      if (p[k] < pairs) {
+        x[k].load(src + p[k] * ss + (uint64_t)c * V);
+        f[k] = w ? w[i * columns + k0 + k] : 1.f;
+      } else {
+        x[k].zero();
+        f[k] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KU; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(f[k], x[k].get(v), acc[v]);
+  }
+  Raw<T, V> r;
+  r.set(acc);
+  r.store(dst + i * ds + (uint64_t)c * V);
+}
+
+// The pair's two rows in one pass: dst[slot] = w * src[token], dw = <src[token],
+// other[slot]>. A group of lanes has a pair, so a token's row is read once
+// from memory and again from the caches for its other choices.
+template <class T, int V, bool DST>
+__global__ void __launch_bounds__(256)
+spread_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint64_t ss, uint32_t columns,
+                  uint64_t pairs, const uint32_t* __restrict__ slot, const float* __restrict__ w,
+                  T* __restrict__ dst, uint64_t ds, const T* __restrict__ other, uint64_t other_s,
+                  float* __restrict__ dw) {
+  constexpr int U = 4;
+  __shared__ float s_sum[8];
+  const uint32_t l = threadIdx.x & (L - 1);
+  const uint64_t pair = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const uint32_t p = pair < pairs ? slot[pair] : kNoSlot;
+  float dot = 0.f;
+  if (p < pairs) {
+    const T* a = src + pair / columns * ss;
+    const T* b = other + p * other_s;
+    const float f = w ? w[pair] : 1.f;
+    for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
+      Raw<T, V> x[U], o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u].zero();
+        o[u].zero();
+        const uint32_t c = c0 + u * L;
+        if (c < chunks) {
+          x[u].load(a + (uint64_t)c * V);
+          o[u].load(b + (uint64_t)c * V);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          dot = fmaf(x[u].get(v), o[u].get(v), dot);
+          y[v] = f * x[u].get(v);
+        }
+        if constexpr (DST) {
+          const uint32_t c = c0 + u * L;
+          if (c < chunks) {
+            if (w) x[u].set(y);
+            x[u].store(dst + p * ds + (uint64_t)c * V);
+          }
+        }
+      }
+    }
+  }
+  dot = group_sum(dot, L, s_sum);
+  if (l == 0 && pair < pairs) dw[pair] = dot;
+}
+
+// dst[i] = sum_c w * src[slot] and dw = <other[i], src[slot]> in one pass, for
+// at most KU choices: a group of lanes has a token.
+template <class T, int V, int KU>
+__global__ void __launch_bounds__(256)
+collect_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint64_t ss, uint64_t n, uint32_t columns,
+                   const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds,
+                   const T* __restrict__ other, uint64_t other_s, float* __restrict__ dw) {
+  __shared__ float s_sum[8];
+  const uint64_t pairs = n * columns;
+  const uint32_t l = threadIdx.x & (L - 1);
+  const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  uint32_t p[KU];
+  float f[KU], dot[KU];
+#pragma unroll
+  for (int k = 0; k < KU; ++k) {
+    const bool in = i < n && (uint32_t)k < columns;
+    p[k] = in ? slot[i * columns + k] : kNoSlot;
+    f[k] = p[k] < pairs ? (w ? w[i * columns + k] : 1.f) : 0.f;
+    dot[k] = 0.f;
+  }
+  if (i < n)
+    for (uint32_t c = l; c < chunks; c += L) {
+      Raw<T, V> o, x[KU];
+      o.load(other + i * other_s + (uint64_t)c * V);
+      float acc[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KU; ++k) {
+        x[k].zero();
+        if (p[k] < pairs) x[k].load(src + p[k] * ss + (uint64_t)c * V);
+      }
+#pragma unroll
+      for (int k = 0; k < KU; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float xv = x[k].get(v);
+          acc[v] = fmaf(f[k], xv, acc[v]);
+          dot[k] = fmaf(o.get(v), xv, dot[k]);
+        }
+      o.set(acc);
+      o.store(dst + i * ds + (uint64_t)c * V);
+    }
+#pragma unroll
+  for (int k = 0; k < KU; ++k) {
+    if ((uint32_t)k >= columns) break;  // the same for the whole grid
+    const float d = group_sum(dot[k], L, s_sum);
+    // a choice that names no row met only zeros, but zero times an infinity is none
+    if (l == 0 && i < n) dw[i * columns + k] = p[k] < pairs ? d : 0.f;
+  }
+}
+
+int spread(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t columns, uint32_t dim,
+           const uint32_t* slot, const float* w, void* dst, uint64_t ds, const void* other, uint64_t os, float* dw) {
+  if (n == 0) return MVR_OK;
+  DeviceScope dev_scope(c);
+  MVR_TRY(dev_scope.status);
+  const uint64_t pairs = n * columns;
+  const int w_ = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {dw ? other : nullptr, os}});
+  return by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return by_vec<T>(w_, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const uint32_t chunks = dim / V;
+      if (dw) {
+        const uint32_t L = lanes_of(c, pairs, chunks);
+        spread_dot_kernel<T, V, true><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(
+            L, chunks, (const T*)src, ss, columns, pairs, slot, w, (T*)dst, ds, (const T*)other, os, dw);
+      } else {
+        const Flat F = flat_of(n, chunks);
+        if (many(c, F))
+          spread_kernel<T, V, 4><<<blocks_of(F.total, 1024), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs,
+                                                                                  slot, w, (T*)dst, ds);
+        else
+          spread_kernel<T, V, 1><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs,
+                                                                                 slot, w, (T*)dst, ds);
+      }
+      MVR_CUDA(c, cudaGetLastError());
+      return (int)MVR_OK;
+    });
+  });
+}
+
+// Choices whose dot products a lane holds at once.
+constexpr uint32_t kDotColumns = 8;
+
+int collect(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t columns, uint32_t dim,
+            const uint32_t* slot, const float* w, void* dst, uint64_t ds, const void* other, uint64_t os, float* dw) {
+  if (n == 0) return MVR_OK;
+  DeviceScope dev_scope(c);
+  MVR_TRY(dev_scope.status);
+  const uint64_t pairs = n * columns;
+  const int w_ = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {dw ? other : nullptr, os}});
+  return by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return by_vec<T>(w_, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const uint32_t chunks = dim / V;
+      const T *s = (const T*)src, *o = (const T*)other;
+      if (dw && columns <= kDotColumns) {
+        const uint32_t L = lanes_of(c, n, chunks);
+        const unsigned blocks = blocks_of(n, 256 / L);
+        if (columns <= 2)
+          collect_dot_kernel<T, V, 2><<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w, (T*)dst,
+                                                                     ds, o, os, dw);
+        else
+          collect_dot_kernel<T, V, kDotColumns><<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w,
+                                                                               (T*)dst, ds, o, os, dw);
+      } else {
+        const Flat F = flat_of(n, chunks);
+        if (columns <= 2)
+          collect_kernel<T, V, 2><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w,
+                                                                                  (T*)dst, ds);
+        else
+          collect_kernel<T, V, 8><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w,
+                                                                                  (T*)dst, ds);
+        if (dw) {  // the dots on their own: src once more
+          const uint32_t L = lanes_of(c, pairs, chunks);
+          spread_dot_kernel<T, V, false><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(
+              L, chunks, o, os, columns, pairs, slot, nullptr, nullptr, 0, s, ss, dw);
+        }
+      }
+      MVR_CUDA(c, cudaGetLastError());
+      return (int)MVR_OK;
+    });
+  });
+}
+
+}  // namespace
+}  // namespace tok
+}  // namespace mvr
+
+using mvr::Ctx;
+
+extern "C" {
+
+int mvr_group_rows_device(mvr_ctx* h, const void* d_x, int dtype, uint64_t x_stride, uint64_t n, uint32_t columns,
+                          uint32_t dim, const uint32_t* d_slot, const float* d_weights, void* d_out,
+                          uint64_t out_stride) {
+  if (!h) return MVR_E_INVALID_ARGUMENT;
+  Ctx* c = &h->impl;
+  MVR_TRY(mvr::tok::check_slots(c, n, columns, d_slot, d_weights));
+  MVR_TRY(mvr::tok::check_rows(c, "x", d_x, dtype, n, dim, x_stride, false));
+  MVR_TRY(mvr::tok::check_rows(c, "out", d_out, dtype, n, dim, out_stride, true));
+  return mvr::tok::spread(c, d_x, dtype, x_stride, n, columns, dim, d_slot, d_weights, d_out, out_stride, nullptr, 0,
+                     nullptr);
+}
+
+int mvr_ungroup_rows_grad_device(mvr_ctx* h, const void* d_dout, int dtype, uint64_t dout_stride, uint64_t n,
+                                 uint32_t columns, uint32_t dim, const uint32_t* d_slot, const float* d_weights,
+                                 const void* d_xs, uint64_t xs_stride, void* d_dxs, uint64_t dxs_stride,
+                                 float* d_dweights) {
+  if (!h) return MVR_E_INVALID_ARGUMENT;
+  Ctx* c = &h->impl;
+  MVR_TRY(mvr::tok::check_slots(c, n, columns, d_slot, d_weights));
+  MVR_TRY(mvr::tok::check_rows(c, "dout", d_dout, dtype, n, dim, dout_stride, false));
+  MVR_TRY(mvr::tok::check_rows(c, "dxs", d_dxs, dtype, n, dim, dxs_stride, true));
+  MVR_TRY(mvr::tok::check_f32(c, "dweights", d_dweights));
+  if (d_dweights) MVR_TRY(mvr::tok::check_rows(c, "xs", d_xs, dtype, n, dim, xs_stride, false));
+  return mvr::tok::spread(c, d_dout, dtype, dout_stride, n, columns, dim, d_slot, d_weights, d_dxs, dxs_stride, d_xs,
+                     xs_stride, d_dweights);
+}
+
+int mvr_ungroup_rows_device(mvr_ctx* h, const void* d_xs, int dtype, uint64_t xs_stride, uint64_t n, uint32_t columns,
+                            uint32_t dim, const uint32_t* d_slot, const float* d_weights, void* d_out,
+                            uint64_t out_stride) {
+  if (!h) return MVR_E_INVALID_ARGUMENT;
+  Ctx* c = &h->impl;
+  MVR_TRY(mvr::tok::check_slots(c, n, columns, d_slot, d_weights));
+  MVR_TRY(mvr::tok::check_rows(c, "xs", d_xs, dtype, n, dim, xs_stride, false));
+  MVR_TRY(mvr::tok::check_rows(c, "out", d_out, dtype, n, dim, out_stride, true));
+  return mvr::tok::collect(c, d_xs, dtype, xs_stride, n, columns, dim, d_slot, d_weights, d_out, out_stride, nullptr, 0,
+                      nullptr);
+}
+
+int mvr_group_rows_grad_device(mvr_ctx* h, const void* d_dout, int dtype, uint64_t dout_stride, uint64_t n,
+                               uint32_t columns, uint32_t dim, const uint32_t* d_slot, const float* d_weights,
+                               const void* d_x, uint64_t x_stride, void* d_dx, uint64_t dx_stride,
+                               float* d_dweights) {
+  if (!h) return MVR_E_INVALID_ARGUMENT;
+  Ctx* c = &h->impl;
+  MVR_TRY(mvr::tok::check_slots(c, n, columns, d_slot, d_weights));
+  MVR_TRY(mvr::tok::check_rows(c, "dout", d_dout, dtype, n, dim, dout_stride, false));
+  MVR_TRY(mvr::tok::check_rows(c, "dx", d_dx, dtype, n, dim, dx_stride, true));
+  MVR_TRY(mvr::tok::check_f32(c, "dweights", d_dweights));
+  if (d_dweights) MVR_TRY(mvr::tok::check_rows(c, "x", d_x, dtype, n, dim, x_stride, false));
+  return mvr::tok::collect(c, d_dout, dtype, dout_stride, n, columns, dim, d_slot, d_weights, d_dx, dx_stride, d_x,
+                      x_stride, d_dweights);
+}
+
+}  // extern "C"

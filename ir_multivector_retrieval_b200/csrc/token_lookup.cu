@@ -1,0 +1,513 @@
+// token_lookup.cu — a table read by token id with scaling, and its gradients by
+// sorted tokens. include/mvr.h states what each call computes.
+#include "token_ops.cuh"
+
+namespace mvr {
+namespace tok {
+namespace {
+
+// ---- lookup ----------------------------------------------------------------
+//
+// Bound by memory: the table's rows that are named are read, every output row
+// is written. One thread per V elements, numbered through the whole output,
+// so that a warp writes one run of memory whatever the row length; four of
+// them a thread, the block's stride apart, when there is work for all SMs.
+
+template <class T, int V, int UR>
+__global__ void __launch_bounds__(256)
+lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, const void* __restrict__ ids,
+              int id_bytes, const float* __restrict__ scale, float alpha, T* __restrict__ out, uint64_t os) {
+  const FlatBlock<UR> B(F);
+  uint64_t i[UR];
+  uint32_t c[UR], r[UR];
+  float f[UR];
+  Raw<T, V> x[UR];
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    r[j] = rows;
+    f[j] = alpha;
+    if (B.at(j, &i[j], &c[j])) {
+      r[j] = row_of(ids, id_bytes, i[j], rows);
+      if (scale) f[j] = alpha * scale[i[j]];
+    } else {
+      i[j] = ~0ull;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    x[j].zero();
+    if (r[j] < rows) x[j].load(table + r[j] * ts + (uint64_t)c[j] * V);
+  }
+#pragma unroll
+  for (int j = 0; j < UR; ++j) {
+    if (i[j] == ~0ull) continue;
+    if (r[j] < rows) {
+      float y[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) y[v] = f[j] * x[j].get(v);
+      x[j].set(y);
+    }
+    x[j].store(out + i[j] * os + (uint64_t)c[j] * V);
+  }
+}
+
+// ---- lookup gradients ------------------------------------------------------
+//
+// dtable is a sum over the sorted places of each key. The places are cut into
+// tiles of one size whatever the keys are, so a key with a seventh of all
+// tokens costs no more time than one with few: a group of L lanes sums Tg
+// consecutive places in registers, 16 bytes of the row a lane, and writes the
+// rows of the keys that begin and end among them. What a key has in a group
+// it does not begin or end in goes through shared memory to the block's other
+// groups, and what it has in a block it does not begin or end in through the
+// workspace to lookup_grad_join_kernel. Every sum's order is fixed by the
+// places, so results do not depend on which block runs first.
+
+// Chunks a lane holds: V elements of a row are at most 16 bytes; rows that
+// cannot be read 16 bytes at a time take several.
+template <class T, int V>
+constexpr int chunks_per_lane() {
+  return (int)sizeof(T) * V >= 16 ? 1 : (int)sizeof(T) * V >= 8 ? 2 : 4;
+}
+
+struct GradShape {
+  uint32_t n, rows, dim;
+  uint32_t lanes;     // L: lanes of a group, a power of two
+  uint32_t per_group;  // Tg: places of a group, a multiple of 8
+  uint64_t gs, ts, ds;  // row strides of grad, table, dtable
+};
+
+template <class T, class O, int V>
+struct GradArgs {
+  GradShape s;
+  const T* grad;
+  const uint32_t *offsets, *order, *keys;
+  const float* scale;
+  float alpha;
+  const T* table;
+  O* dtable;
+  int accumulate;
+  float* dscale;
+  float* part;  // [tile][2][dim]: 0 the end of a key that began before the tile, 1 what goes on behind it
+};
+
+template <class O, int V>
+__device__ __forceinline__ void put_sum(O* p, const float (&sum)[V], int accumulate) {
+  Raw<O, V> r;
+  if (accumulate) {
+    float x[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = to_f32(p[v]) + sum[v];
+    r.set(x);
+  } else {
+    r.set(sum);
+  }
+  r.store(p);
+}
+
+template <class T, class O, int V, bool DSCALE>
+__global__ void __launch_bounds__(256)
+lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
+  constexpr int NCH = chunks_per_lane<T, V>();
+  constexpr int U = DSCALE ? 4 : 8;  // rows in flight a lane
+  __shared__ float s_head[256 * NCH * V], s_tail[256 * NCH * V];
+  __shared__ uint8_t s_hkind[256], s_has_tail[256];  // head: 0 none, 1 ends here, 2 goes on
+  __shared__ uint32_t s_hkey[256], s_tkey[256];
+  const GradShape& S = A.s;
+  const uint32_t L = S.lanes, G = 256 / L;
+  const uint32_t g = threadIdx.x / L, l = threadIdx.x & (L - 1);
+  const uint32_t valid = min(A.offsets[S.rows], S.n);
+  const uint32_t tile = G * S.per_group;
+  const uint64_t tile0 = (uint64_t)blockIdx.x * tile;
+  if constexpr (DSCALE) {  // the tokens behind the last place name no row
+    const uint64_t end = min((uint64_t)S.n, tile0 + tile);
+    for (uint64_t p = max((uint64_t)valid, tile0) + threadIdx.x; p < end; p += 256)
+      if (A.order[p] < S.n) A.dscale[A.order[p]] = 0.f;
+  }
+  if (tile0 >= valid) return;
+  const uint32_t a = (uint32_t)min((uint64_t)valid, tile0 + (uint64_t)g * S.per_group);
+  const uint32_t b = (uint32_t)min((uint64_t)valid, tile0 + (uint64_t)(g + 1) * S.per_group);
+  uint32_t col[NCH];
+  bool on[NCH];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    col[k] = ((blockIdx.y * NCH + k) * L + l) * V;
+    on[k] = col[k] < S.dim;
+  }
+  float acc[NCH][V];
+  auto clear = [&]() {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[k][v] = 0.f;
+  };
+  clear();
+
+  bool started = a < b && (a == 0 || A.keys[a - 1] != A.keys[a]);
+  uint32_t cur = a < b ? A.keys[a] : S.rows;
+  uint32_t hkind = 0;
+  auto stage = [&](float* where) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) where[((g * NCH + k) * V + v) * L + l] = acc[k][v];
+  };
+  auto write = [&](uint32_t key) {
+    if (key < S.rows)
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+        if (on[k]) put_sum(A.dtable + (uint64_t)key * S.ds + col[k], acc[k], A.accumulate);
+  };
+
+  const uint32_t steps = (S.per_group + U - 1) / U;  // the same for all lanes: shuffles inside
+  for (uint32_t step = 0; step < steps; ++step) {
+    const uint32_t p0 = a + step * U;
+    if (__all_sync(0xffffffffu, p0 >= b)) break;
+    uint32_t key[U], tok[U];
+    float f[U];
+    Raw<T, V> row[U][NCH], trow[DSCALE ? U : 1][NCH];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = p0 + u < b;
+      key[u] = in ? A.keys[p0 + u] : S.rows;
+      tok[u] = in ? A.order[p0 + u] : S.n;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = tok[u] < S.n && key[u] < S.rows;
+      f[u] = in ? (A.scale ? A.alpha * A.scale[tok[u]] : A.alpha) : 0.f;
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        row[u][k].zero();
+        if (in && on[k]) row[u][k].load(A.grad + tok[u] * S.gs + col[k]);
+        if constexpr (DSCALE) {
+          trow[u][k].zero();
+          if (in && on[k]) trow[u][k].load(A.table + key[u] * S.ts + col[k]);
+        }
+      }
+    }
+    if constexpr (DSCALE) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float dot = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+          for (int v = 0; v < V; ++v) dot = fmaf(row[u][k].get(v), trow[u][k].get(v), dot);
+        for (uint32_t o = L >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (l == 0 && tok[u] < S.n) A.dscale[tok[u]] = A.alpha * dot;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p0 + u < b) {
+        if (key[u] != cur) {
+          if (started) {
+            write(cur);
+          } else {
+            stage(s_head);
+            hkind = 1;
+            if (l == 0) s_hkey[g] = cur;
+          }
+          started = true;
+          cur = key[u];
+          clear();
+        }
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[k][v] = fmaf(f[u], row[u][k].get(v), acc[k][v]);
+      }
+    }
+  }
+  bool has_tail = false;
+  if (a < b) {
+    const bool ends = b == valid || A.keys[b] != cur;
+    if (started && ends) {
+      write(cur);
+    } else if (!started) {
+      stage(s_head);
+      hkind = ends ? 1 : 2;
+      if (l == 0) s_hkey[g] = cur;
+    } else {
+      stage(s_tail);
+      has_tail = true;
+      if (l == 0) s_tkey[g] = cur;
+    }
+  }
+  if (l == 0) {
+    s_hkind[g] = (uint8_t)hkind;
+    s_has_tail[g] = has_tail;
+  }
+  __syncthreads();
+
+  // a group that began a key which goes on adds what the next groups have of
+  // it; the first group does the same for a key that began in an earlier block
+  const bool from_before = g == 0 && s_hkind[0] != 0;
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+    if (turn == 0 ? !from_before : !s_has_tail[g]) continue;
+    const uint32_t key = turn == 0 ? s_hkey[0] : s_tkey[g];
+    const float* first = turn == 0 ? s_head : s_tail;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[k][v] = first[((g * NCH + k) * V + v) * L + l];
+    bool open = turn == 1 || s_hkind[0] == 2;
+    for (uint32_t q = g + 1; open && q < G && s_hkind[q] != 0; ++q) {
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[k][v] += s_head[((q * NCH + k) * V + v) * L + l];
+      open = s_hkind[q] == 2;
+    }
+    if (turn == 1 && !open) {
+      write(key);
+    } else {
+      float* out = A.part + ((uint64_t)blockIdx.x * 2 + (open ? 1 : 0)) * S.dim;
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+        if (on[k])
+#pragma unroll
+          for (int v = 0; v < V; ++v) out[col[k] + v] = acc[k][v];
+    }
+  }
+}
+
+// Rows without a token become zeros (blocks from `joins` on), and block t <
+// joins sums the key that crosses the border of tiles t and t + 1 and has
+// crossed no earlier one: what it left behind the tiles, in their order, then
+// its end.
+template <class O, int V>
+__global__ void __launch_bounds__(256)
+lookup_grad_join_kernel(GradShape S, uint32_t tile, uint32_t joins, const uint32_t* __restrict__ offsets,
+                        const uint32_t* __restrict__ keys, const float* __restrict__ part, O* __restrict__ dtable,
+                        int accumulate) {
+  if (blockIdx.x >= joins) {
+    if (accumulate) return;
+    const uint32_t chunks = S.dim / V;
+    const uint64_t total = (uint64_t)S.rows * chunks;
+    for (uint64_t e = (uint64_t)(blockIdx.x - joins) * 256 + threadIdx.x; e < total;
+         e += (uint64_t)(gridDim.x - joins) * 256) {
+      const uint32_t v = (uint32_t)(e / chunks), c = (uint32_t)(e - (uint64_t)v * chunks);
+      if (offsets[v] == offsets[v + 1]) {
+        Raw<O, V> z;
+        z.zero();
+        z.store(dtable + v * S.ds + c * V);
+      }
+    }
+    return;
+  }
+  const uint32_t valid = min(offsets[S.rows], S.n);
+  const uint64_t border = (uint64_t)(blockIdx.x + 1) * tile;
+  if (border >= valid) return;
+  const uint32_t key = keys[border];
+  if (key >= S.rows || keys[border - 1] != key) return;
+  const uint32_t first = offsets[key] / tile, last = (min(offsets[key + 1], valid) - 1) / tile;
+  if (first != blockIdx.x) return;
+  __shared__ float s_sum[256];
+  // 32 columns at a time, 8 warps over the tiles
+  const uint32_t w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  for (uint32_t c0 = 0; c0 < S.dim; c0 += 32) {
+    const uint32_t c = c0 + l;
+    float acc = 0.f;
+    if (c < S.dim) {
+#pragma unroll 8
+      for (uint32_t t = first + w; t < last; t += 8) acc += part[((uint64_t)t * 2 + 1) * S.dim + c];
+    }
+    s_sum[threadIdx.x] = acc;
+    __syncthreads();
+    if (w == 0 && c < S.dim) {
+#pragma unroll
+      for (int q = 1; q < 8; ++q) acc += s_sum[q * 32 + l];
+      acc += part[(uint64_t)last * 2 * S.dim + c];
+      O* o = dtable + (uint64_t)key * S.ds + c;
+      *o = from_f32<O>(accumulate ? to_f32(*o) + acc : acc);
+    }
+    __syncthreads();
+  }
+}
+
+// dscale where a row's parts lie in several blocks of the sums: a group of L
+// lanes per token, its table row is the key at its place.
+template <class T, int V>
+__global__ void __launch_bounds__(256)
+lookup_dscale_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ grad, uint64_t gs, uint32_t n, uint32_t rows,
+                     const uint32_t* __restrict__ keys, const uint32_t* __restrict__ slot, float alpha,
+                     const T* __restrict__ table, uint64_t ts, float* __restrict__ dscale) {
+  constexpr int U = 4;
+  __shared__ float s_sum[8];
+  const uint32_t l = threadIdx.x & (L - 1);
+  const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const uint32_t p = i < n ? slot[i] : kNoSlot, r = p < n ? keys[p] : rows;
+  float dot = 0.f;
+  if (r < rows) {
+    const T* a = grad + i * gs;
+    const T* b = table + r * ts;
+    for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
+      Raw<T, V> x[U], o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u].zero();
+        o[u].zero();
+        const uint32_t c = c0 + u * L;
+        if (c < chunks) {
+          x[u].load(a + (uint64_t)c * V);
+          o[u].load(b + (uint64_t)c * V);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) dot = fmaf(x[u].get(v), o[u].get(v), dot);
+    }
+  }
+  dot = group_sum(dot, L, s_sum);
+  if (l == 0 && i < n) dscale[i] = alpha * dot;
+}
+
+// Smallest block of places, whatever the row length: the workspace is sized
+// for it. 8 places a group, 8 groups of 32 lanes at least.
+constexpr uint32_t kMinTile = 64;
+
+template <class T, class O, int V>
+int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
+  GradShape& S = A.s;
+  cudaStream_t st = c->stream;
+  constexpr uint32_t NCH = chunks_per_lane<T, V>();
+  const uint32_t chunks = S.dim / V;
+  S.lanes = std::min(32u, pow2_ceil((chunks + NCH - 1) / NCH));
+  const uint32_t slabs = (chunks + S.lanes * NCH - 1) / (S.lanes * NCH);
+  const uint32_t groups = 256 / S.lanes;
+  // Long groups leave fewer sums to join, short ones more blocks: the longest
+  // of 8 to 64 places that still gives every SM eight blocks.
+  S.per_group = 64;
+  while (S.per_group > 8 &&
+         (uint64_t)slabs * ((S.n + (uint64_t)groups * S.per_group - 1) / ((uint64_t)groups * S.per_group)) <
+             8ull * c->sm_count)
+    S.per_group >>= 1;
+  const uint32_t tile = groups * S.per_group;
+  const uint32_t tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
+  if (tiles) {
+    if (A.dscale && slabs == 1)
+      lookup_grad_tile_kernel<T, O, V, true><<<dim3(tiles, slabs), 256, 0, st>>>(A);
+    else
+      lookup_grad_tile_kernel<T, O, V, false><<<dim3(tiles, slabs), 256, 0, st>>>(A);
+    if (A.dscale && slabs > 1) {  // a row's parts lie in several blocks
+      const uint32_t L = lanes_of(c, S.n, chunks);
+      lookup_dscale_kernel<T, V><<<blocks_of(S.n, 256 / L), 256, 0, st>>>(
+          L, chunks, A.grad, S.gs, S.n, S.rows, A.keys, slot, A.alpha, A.table, S.ts, A.dscale);
+    }
+  }
+  const uint32_t joins = tiles ? tiles - 1 : 0;
+  const uint64_t fill = A.accumulate ? 0 : std::min<uint64_t>(((uint64_t)S.rows * chunks + 255) / 256, 8ull * c->sm_count);
+  if (joins + fill)
+    lookup_grad_join_kernel<O, V><<<(unsigned)(joins + fill), 256, 0, st>>>(S, tile, joins, A.offsets, A.keys, A.part,
+                                                                           A.dtable, A.accumulate);
+  MVR_CUDA(c, cudaGetLastError());
+  return MVR_OK;
+}
+
+}  // namespace
+}  // namespace tok
+}  // namespace mvr
+
+using mvr::Ctx;
+
+extern "C" {
+
+int mvr_lookup_device(mvr_ctx* h, const void* d_table, int dtype, uint64_t rows, uint32_t dim, uint64_t table_stride,
+                      const void* d_ids, int id_bytes, uint64_t n, const float* d_scale, float alpha, void* d_out,
+                      uint64_t out_stride) {
+  if (!h) return MVR_E_INVALID_ARGUMENT;
+  Ctx* c = &h->impl;
+  MVR_TRY(mvr::tok::check_rows(c, "table", d_table, dtype, rows, dim, table_stride, false));
+  MVR_TRY(mvr::tok::check_ids(c, d_ids, id_bytes, n, rows));
+  MVR_TRY(mvr::tok::check_rows(c, "out", d_out, dtype, n, dim, out_stride, true));
+  MVR_TRY(mvr::tok::check_f32(c, "scale", d_scale));
+  if (n == 0) return MVR_OK;
+  mvr::DeviceScope dev_scope(c);
+  MVR_TRY(dev_scope.status);
+  const int w = mvr::tok::vec_of(dtype, dim, {{d_table, table_stride}, {d_out, out_stride}});
+  return mvr::tok::by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return mvr::tok::by_vec<T>(w, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const mvr::tok::Flat F = mvr::tok::flat_of(n, dim / V);
+      if (mvr::tok::many(c, F))
+        mvr::tok::lookup_kernel<T, V, 4><<<mvr::tok::blocks_of(F.total, 1024), 256, 0, c->stream>>>(
+            F, (const T*)d_table, (uint32_t)rows, table_stride, d_ids, id_bytes, d_scale, alpha, (T*)d_out,
+            out_stride);
+      else
+        mvr::tok::lookup_kernel<T, V, 1><<<mvr::tok::blocks_of(F.total, 256), 256, 0, c->stream>>>(
+            F, (const T*)d_table, (uint32_t)rows, table_stride, d_ids, id_bytes, d_scale, alpha, (T*)d_out,
+            out_stride);
+      MVR_CUDA(c, cudaGetLastError());
+      return (int)MVR_OK;
+    });
+  });
+}
+
+int mvr_lookup_grad_bytes(uint64_t n_ids, uint32_t dim, uint64_t* bytes) {
+  if (!bytes || n_ids > mvr::tok::kMaxIds || dim == 0) return MVR_E_INVALID_ARGUMENT;
+  *bytes = (n_ids + mvr::tok::kMinTile - 1) / mvr::tok::kMinTile * 2 * dim * sizeof(float);
+  return MVR_OK;
+}
+
+int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t grad_stride, uint64_t n_ids,
+                           uint64_t rows, uint32_t dim, const uint32_t* d_offsets, const uint32_t* d_order,
+                           const uint32_t* d_keys, const uint32_t* d_slot, const float* d_scale, float alpha,
+                           const void* d_table, uint64_t table_stride, void* d_dtable, int dtable_dtype,
+                           uint64_t dtable_stride, int accumulate, float* d_dscale, void* d_workspace,
+                           uint64_t workspace_bytes) {
+  if (!h) return MVR_E_INVALID_ARGUMENT;
+  Ctx* c = &h->impl;
+  MVR_TRY(mvr::tok::check_rows(c, "grad", d_grad, dtype, n_ids, dim, grad_stride, false));
+  if (rows == 0 || rows > mvr::tok::kMaxRows) return mvr::tok::bad(c, "rows must be in [1, 2^31 - 2]");
+  if (n_ids > mvr::tok::kMaxIds) return mvr::tok::bad(c, "more than 2^31 - 1 ids");
+  if (dtable_dtype != dtype && dtable_dtype != MVR_F32) return mvr::tok::bad(c, "dtable must have grad's type or f32");
+  MVR_TRY(mvr::tok::check_rows(c, "dtable", d_dtable, dtable_dtype, rows, dim, dtable_stride, true));
+  if (!d_offsets || (n_ids && (!d_order || !d_keys || !d_slot))) return mvr::tok::bad(c, "null pointer: plan");
+  if (!mvr::tok::aligned(d_offsets, 4) || !mvr::tok::aligned(d_order, 4) || !mvr::tok::aligned(d_keys, 4) || !mvr::tok::aligned(d_slot, 4))
+    return mvr::tok::bad(c, "the plan is not aligned to its type");
+  MVR_TRY(mvr::tok::check_f32(c, "scale", d_scale));
+  MVR_TRY(mvr::tok::check_f32(c, "dscale", d_dscale));
+  if (d_dscale) MVR_TRY(mvr::tok::check_rows(c, "table", d_table, dtype, rows, dim, table_stride, false));
+  uint64_t need = 0;
+  MVR_TRY(mvr_lookup_grad_bytes(n_ids, dim, &need));
+  MVR_TRY(mvr::tok::check_workspace(c, d_workspace, workspace_bytes, need));
+  mvr::DeviceScope dev_scope(c);
+  MVR_TRY(dev_scope.status);
+  const uint32_t n = (uint32_t)n_ids, v = (uint32_t)rows;
+  return mvr::tok::by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    auto run = [&](auto* o) {
+      using O = std::remove_pointer_t<decltype(o)>;
+      int w = mvr::tok::vec_of(dtype, dim, {{d_grad, grad_stride}, {d_dscale ? d_table : nullptr, table_stride}});
+      // 8 f32 sums are two 16-byte accesses, so 16-byte alignment serves them too
+      const int wo = mvr::tok::vec_of(dtable_dtype, dim, {{d_dtable, dtable_stride}});
+      w = std::min(w, sizeof(O) > sizeof(T) && wo == 4 ? 8 : wo);
+      return mvr::tok::by_vec<T>(w, [&](auto vec) {
+        constexpr int V = decltype(vec)::value;
+        mvr::tok::GradArgs<T, O, V> A;
+        A.s = {n, v, dim, 0, 0, grad_stride, table_stride, dtable_stride};
+        A.grad = (const T*)d_grad;
+        A.offsets = d_offsets;
+        A.order = d_order;
+        A.keys = d_keys;
+        A.scale = d_scale;
+        A.alpha = alpha;
+        A.table = (const T*)d_table;
+        A.dtable = (O*)d_dtable;
+        A.accumulate = accumulate;
+        A.dscale = d_dscale;
+        A.part = (float*)d_workspace;
+        return mvr::tok::lookup_grad_run(c, A, d_slot);
+      });
+    };
+    if (dtable_dtype == MVR_F32) return run(static_cast<float*>(nullptr));
+    return run(t);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,452 @@
+// token_plan.cu — the stable sort of token ids that the table's gradient and
+// the grouping of rows read. include/mvr.h states what it gives.
+#include <cooperative_groups.h>
+
+#include "token_ops.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace mvr {
+namespace tok {
+namespace {
+
+// The sort is by radix, stable: in each pass, least significant digit first, a
+// pair goes to (pairs of smaller digits) + (pairs of its digit before it). The
+// ids are a few bytes a token beside rows of hundreds, so what costs is the
+// number of dependent steps: up to kSmallMax pairs one cluster of blocks does
+// all passes in one launch; above, a pass is three launches over tiles.
+
+constexpr uint32_t kSmallThreads = 1024, kSmallRounds = 8, kSmallBlocks = 8;
+constexpr uint32_t kSmallMax = kSmallThreads * kSmallRounds * kSmallBlocks;  // 65,536 pairs
+constexpr int kSmallBits = 9;                                                // of a digit
+constexpr uint32_t kTileThreads = 256, kTileRounds = 16, kTile = kTileThreads * kTileRounds;
+constexpr int kTileBits = 10;
+
+struct PlanArgs {
+  const void* ids;
+  int id_bytes;
+  uint32_t n, rows;
+  uint32_t *offsets, *order, *keys, *slot;
+};
+
+// Equal digits among the warp's lanes: how many are below this lane, and
+// whether it is the first.
+struct Peers {
+  uint32_t below, count;
+  __device__ __forceinline__ explicit Peers(uint32_t digit) {
+    const uint32_t m = __match_any_sync(0xffffffffu, digit);
+    below = __popc(m & lanemask_lt());
+    count = __popc(m);
+  }
+};
+
+// Exclusive prefix sums of s[0 .. R), R a power of two up to 4 a thread, by all
+// `threads` threads of the block (a multiple of 32, at most 1024). w: one value
+// a warp.
+__device__ __forceinline__ void block_prefix(uint32_t* s, uint32_t R, uint32_t threads, uint32_t* w) {
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint32_t per = R <= threads ? 1 : R / threads;
+  uint32_t v[4], sum = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    v[k] = k < per && t * per + k < R ? s[t * per + k] : 0;
+    sum += v[k];
+  }
+  uint32_t run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= (uint32_t)o) run += x;
+  }
+  if (lane == 31) w[warp] = run;
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t x = lane < threads / 32 ? w[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= (uint32_t)o) x += y;
+    }
+    w[lane] = x;
+  }
+  __syncthreads();
+  run += (warp ? w[warp - 1] : 0) - sum;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k)
+    if (k < per && t * per + k < R) {
+      s[t * per + k] = run;
+      run += v[k];
+    }
+  __syncthreads();
+}
+
+// All passes over at most kSmallMax pairs by one cluster. Block c has the
+// pairs [c * chunk, (c + 1) * chunk), a warp 32 x rounds of them in order, and
+// the blocks read one another's digit counts from shared memory. With one
+// pass the digits are the keys, and their prefix sums the offsets.
+__global__ void __launch_bounds__(kSmallThreads)
+plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint32_t* k0, uint32_t* v0, uint32_t* k1,
+                  uint32_t* v1) {
+  __shared__ uint16_t s_count[32][1 << kSmallBits];  // a warp's pairs of a digit; then those of the warps before
+  __shared__ uint32_t s_total[1 << kSmallBits], s_base[1 << kSmallBits], s_warp[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint32_t R = 1u << digit_bits;
+  const uint32_t first = rank * (rounds * kSmallThreads) + warp * (rounds * 32) + lane;
+  const uint32_t *kin = nullptr, *vin = nullptr;
+  uint32_t *kout = k0, *vout = v0;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit_bits;
+    const bool last = pass + 1 == passes;
+    for (uint32_t e = t; e < 32 * R; e += kSmallThreads) s_count[e >> digit_bits][e & (R - 1)] = 0;
+    uint32_t key[kSmallRounds], val[kSmallRounds], place[kSmallRounds];
+#pragma unroll
+    for (uint32_t j = 0; j < kSmallRounds; ++j) {
+      const uint32_t e = first + j * 32;
+      key[j] = val[j] = 0;
+      if (j < rounds && e < A.n) {
+        key[j] = pass ? __ldcg(kin + e) : row_of(A.ids, A.id_bytes, e, A.rows);
+        val[j] = pass ? __ldcg(vin + e) : e;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kSmallRounds; ++j) {
+      if (j >= rounds) break;
+      const bool in = first + j * 32 < A.n;
+      const uint32_t d = (key[j] >> shift) & (R - 1);
+      const Peers p(in ? d : R + lane);
+      if (in) place[j] = s_count[warp][d] + p.below;
+      __syncwarp();
+      if (in && p.below == 0) s_count[warp][d] += (uint16_t)p.count;
+      __syncwarp();
+    }
+    __syncthreads();
+    if (t < R) {
+      uint32_t run = 0;
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        const uint32_t x = s_count[q][t];
+        s_count[q][t] = (uint16_t)run;
+        run += x;
+      }
+      s_total[t] = run;
+    }
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    if (t < R) {
+      for (uint32_t q = 0; q < blocks; ++q) {
+        const uint32_t x = *cluster.map_shared_rank(&s_total[t], q);
+        if (q < rank) before += x;
+        all += x;
+      }
+      s_base[t] = all;
+    }
+    __syncthreads();
+    block_prefix(s_base, R, kSmallThreads, s_warp);
+    if (t < R) {
+      if (passes == 1 && rank == 0 && t <= A.rows) A.offsets[t] = s_base[t];
+      s_base[t] += before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kSmallRounds; ++j) {
+      if (j >= rounds || first + j * 32 >= A.n) break;
+      const uint32_t d = (key[j] >> shift) & (R - 1);
+      const uint32_t pos = s_base[d] + s_count[warp][d] + place[j];
+      if (last) {
+        A.keys[pos] = key[j];
+        A.order[pos] = val[j];
+        A.slot[val[j]] = key[j] < A.rows ? pos : kNoSlot;
+      } else {
+        __stcg(kout + pos, key[j]);
+        __stcg(vout + pos, val[j]);
+      }
+    }
+    cluster.sync();  // the pairs are in place, and nobody reads this block's counts any more
+    kin = kout;
+    vin = vout;
+    kout = kout == k0 ? k1 : k0;
+    vout = vout == v0 ? v1 : v0;
+  }
+}
+
+// Pairs of each digit in a tile: hist[digit][tile].
+__global__ void __launch_bounds__(kTileThreads)
+plan_hist_kernel(PlanArgs A, const uint32_t* __restrict__ kin, int shift, uint32_t R, uint32_t tiles,
+                 uint32_t* __restrict__ hist) {
+  __shared__ uint32_t s_count[1 << kTileBits];
+  grid_dependency_wait();
+  const uint32_t t = threadIdx.x;
+  for (uint32_t d = t; d < R; d += kTileThreads) s_count[d] = 0;
+  __syncthreads();
+  const uint64_t first = (uint64_t)blockIdx.x * kTile + t;
+#pragma unroll
+  for (uint32_t j = 0; j < kTileRounds; ++j) {
+    const uint64_t e = first + j * kTileThreads;
+    if (e < A.n) {
+      const uint32_t key = kin ? kin[e] : row_of(A.ids, A.id_bytes, e, A.rows);
+      atomicAdd(&s_count[(key >> shift) & (R - 1)], 1u);
+    }
+  }
+  __syncthreads();
+  for (uint32_t d = t; d < R; d += kTileThreads) hist[(uint64_t)d * tiles + blockIdx.x] = s_count[d];
+}
+
+// A digit's counts become those of the tiles before; its total beside them.
+__global__ void __launch_bounds__(256)
+plan_scan_kernel(uint32_t tiles, uint32_t* __restrict__ hist, uint32_t* __restrict__ total) {
+  __shared__ uint32_t s_part[1024], s_warp[32];
+  grid_dependency_wait();
+  uint32_t* h = hist + (uint64_t)blockIdx.x * tiles;
+  uint32_t run = 0;
+  for (uint32_t t0 = 0; t0 < tiles; t0 += 1024) {
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint32_t t = t0 + k * 256 + threadIdx.x;
+      s_part[k * 256 + threadIdx.x] = t < tiles ? h[t] : 0;
+    }
+    __syncthreads();
+    const uint32_t end = s_part[1023];
+    block_prefix(s_part, 1024, 256, s_warp);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      const uint32_t t = t0 + k * 256 + threadIdx.x;
+      if (t < tiles) h[t] = run + s_part[k * 256 + threadIdx.x];
+    }
+    run += s_part[1023] + end;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) total[blockIdx.x] = run;
+}
+
+// A tile's pairs, sorted by digit in shared memory first so that each digit's
+// run is written in one piece.
+template <bool LAST>
+__global__ void __launch_bounds__(kTileThreads)
+plan_scatter_kernel(PlanArgs A, const uint32_t* __restrict__ kin, const uint32_t* __restrict__ vin, int shift,
+                    uint32_t R, uint32_t tiles, const uint32_t* __restrict__ hist,
+                    const uint32_t* __restrict__ total, uint32_t* __restrict__ kout, uint32_t* __restrict__ vout) {
+  constexpr uint32_t kWarps = kTileThreads / 32;
+  extern __shared__ uint32_t smem[];
+  uint32_t* s_key = smem;              // [kTile]
+  uint32_t* s_val = s_key + kTile;     // [kTile]
+  uint32_t* s_start = s_val + kTile;   // [R] first place of the digit in the tile
+  uint32_t* s_glob = s_start + R;      // [R] its first place among all, less s_start
+  uint16_t* s_count = reinterpret_cast<uint16_t*>(s_glob + R);  // [kWarps][R]
+  __shared__ uint32_t s_warp[32];
+  grid_dependency_wait();
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  for (uint32_t e = t; e < kWarps * R; e += kTileThreads) s_count[e] = 0;
+  for (uint32_t d = t; d < R; d += kTileThreads) s_glob[d] = total[d];
+  const uint64_t tile0 = (uint64_t)blockIdx.x * kTile;
+  const uint32_t in_tile = (uint32_t)min((uint64_t)kTile, A.n - tile0);
+  const uint32_t first = warp * (kTileRounds * 32) + lane;
+  uint32_t key[kTileRounds], val[kTileRounds], place[kTileRounds];
+#pragma unroll
+  for (uint32_t j = 0; j < kTileRounds; ++j) {
+    const uint32_t q = first + j * 32;
+    key[j] = val[j] = 0;
+    if (q < in_tile) {
+      key[j] = kin ? kin[tile0 + q] : row_of(A.ids, A.id_bytes, tile0 + q, A.rows);
+      val[j] = vin ? vin[tile0 + q] : (uint32_t)(tile0 + q);
+    }
+  }
+  __syncthreads();
+  block_prefix(s_glob, R, kTileThreads, s_warp);
+  uint16_t* mine = s_count + warp * R;
+#pragma unroll
+  for (uint32_t j = 0; j < kTileRounds; ++j) {
+    const bool in = first + j * 32 < in_tile;
+    const uint32_t d = (key[j] >> shift) & (R - 1);
+    const Peers p(in ? d : R + lane);
+    if (in) place[j] = mine[d] + p.below;
+    __syncwarp();
+    if (in && p.below == 0) mine[d] += (uint16_t)p.count;
+    __syncwarp();
+  }
+  __syncthreads();
+  for (uint32_t d = t; d < R; d += kTileThreads) {
+    uint32_t run = 0;
+#pragma unroll
+    for (uint32_t q = 0; q < kWarps; ++q) {
+      const uint32_t x = s_count[q * R + d];
+      s_count[q * R + d] = (uint16_t)run;
+      run += x;
+    }
+    s_start[d] = run;
+  }
+  __syncthreads();
+  block_prefix(s_start, R, kTileThreads, s_warp);
+  for (uint32_t d = t; d < R; d += kTileThreads)
+    s_glob[d] += hist[(uint64_t)d * tiles + blockIdx.x] - s_start[d];
+#pragma unroll
+  for (uint32_t j = 0; j < kTileRounds; ++j) {
+    if (first + j * 32 < in_tile) {
+      const uint32_t d = (key[j] >> shift) & (R - 1);
+      const uint32_t q = s_start[d] + mine[d] + place[j];
+      s_key[q] = key[j];
+      s_val[q] = val[j];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t j = 0; j < kTileRounds; ++j) {
+    const uint32_t q = j * kTileThreads + t;
+    if (q >= in_tile) break;
+    const uint32_t k = s_key[q], v = s_val[q];
+    const uint32_t pos = s_glob[(k >> shift) & (R - 1)] + q;
+    if (LAST) {
+      A.keys[pos] = k;
+      A.order[pos] = v;
+      A.slot[v] = k < A.rows ? pos : kNoSlot;
+    } else {
+      kout[pos] = k;
+      vout[pos] = v;
+    }
+  }
+}
+
+// offsets[v] = first place whose key is >= v, by bisection.
+__global__ void __launch_bounds__(256) plan_offsets_kernel(PlanArgs A) {
+  grid_dependency_wait();
+  const uint32_t v = blockIdx.x * 256u + threadIdx.x;
+  if (v > A.rows) return;
+  uint32_t lo = 0, hi = A.n;
+  while (lo < hi) {
+    const uint32_t mid = lo + ((hi - lo) >> 1);
+    if (A.keys[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  A.offsets[v] = lo;
+}
+
+struct Digits {
+  int bits, passes;
+  Digits(uint64_t rows, int most) {
+    int b = 1;
+    while ((rows >> b) != 0) ++b;  // keys are 0 .. rows
+    passes = (b + most - 1) / most;
+    bits = (b + passes - 1) / passes;
+  }
+};
+
+// Workspace: two sets of pairs for the passes, and the counts of the tiles.
+struct PlanSpace {
+  uint64_t k0, v0, k1, v1, hist, sums, total;
+  PlanSpace(uint64_t n, uint64_t rows) {
+    const bool small = n <= kSmallMax;
+    const Digits D(rows, small ? kSmallBits : kTileBits);
+    uint64_t off = 0;
+    auto take = [&](uint64_t words) {
+      const uint64_t o = off;
+      off += up256(words * 4);
+      return o;
+    };
+    k0 = take(D.passes > 1 ? n : 0);
+    v0 = take(D.passes > 1 ? n : 0);
+    k1 = take(D.passes > 2 ? n : 0);
+    v1 = take(D.passes > 2 ? n : 0);
+    hist = take(small ? 0 : ((n + kTile - 1) / kTile) << D.bits);
+    sums = take(small ? 0 : 1ull << D.bits);
+    total = off;
+  }
+};
+
+int plan_small(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_t* v0, uint32_t* k1, uint32_t* v1) {
+  // 2048 pairs a block and more before another block joins
+  const uint32_t blocks = std::min(kSmallBlocks, pow2_ceil((A.n + 2047) / 2048));
+  const uint32_t chunk = (A.n + blocks - 1) / blocks;
+  const uint32_t rounds = (chunk + kSmallThreads - 1) / kSmallThreads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = blocks;
+  cfg.blockDim = kSmallThreads;
+  cfg.stream = c->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MVR_CUDA(c, cudaLaunchKernelEx(&cfg, plan_small_kernel, A, rounds, D.bits, D.passes, k0, v0, k1, v1));
+  return MVR_OK;
+}
+
+int plan_tiles(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_t* v0, uint32_t* k1, uint32_t* v1,
+               uint32_t* hist, uint32_t* sums) {
+  cudaStream_t st = c->stream;
+  const uint32_t tiles = (A.n + (kTile - 1ull)) / kTile, R = 1u << D.bits;
+  const size_t smem = (2 * kTile + 2 * R) * 4 + kTileThreads / 32 * R * 2;
+  MVR_CUDA(c, raise_smem_limit((const void*)plan_scatter_kernel<true>, smem));
+  MVR_CUDA(c, raise_smem_limit((const void*)plan_scatter_kernel<false>, smem));
+  const uint32_t *kin = nullptr, *vin = nullptr;
+  uint32_t *kout = k0, *vout = v0;
+  for (int pass = 0; pass < D.passes; ++pass) {
+    const int shift = pass * D.bits;
+    MVR_CUDA(c, launch_pdl(plan_hist_kernel, tiles, kTileThreads, 0, st, A, kin, shift, R, tiles, hist));
+    MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
+    const auto scatter = pass + 1 == D.passes ? plan_scatter_kernel<true> : plan_scatter_kernel<false>;
+    MVR_CUDA(c, launch_pdl(scatter, tiles, kTileThreads, smem, st, A, kin, vin, shift, R, tiles, hist, sums, kout,
+                           vout));
+    kin = kout;
+    vin = vout;
+    kout = kout == k0 ? k1 : k0;
+    vout = vout == v0 ? v1 : v0;
+  }
+  return MVR_OK;
+}
+
+}  // namespace
+}  // namespace tok
+}  // namespace mvr
+
+using mvr::Ctx;
+
+extern "C" {
+
+int mvr_token_plan_bytes(uint64_t n_ids, uint64_t rows, uint64_t* bytes) {
+  if (!bytes || n_ids > mvr::tok::kMaxIds || rows == 0 || rows > mvr::tok::kMaxRows) return MVR_E_INVALID_ARGUMENT;
+  *bytes = n_ids ? mvr::tok::PlanSpace(n_ids, rows).total : 0;
+  return MVR_OK;
+}
+
+int mvr_token_plan_device(mvr_ctx* h, const void* d_ids, int id_bytes, uint64_t n_ids, uint64_t rows,
+                          uint32_t* d_offsets, uint32_t* d_order, uint32_t* d_keys, uint32_t* d_slot,
+                          void* d_workspace, uint64_t workspace_bytes) {
+  if (!h) return MVR_E_INVALID_ARGUMENT;
+  Ctx* c = &h->impl;
+  MVR_TRY(mvr::tok::check_ids(c, d_ids, id_bytes, n_ids, rows));
+  if (n_ids > mvr::tok::kMaxIds) return mvr::tok::bad(c, "more than 2^31 - 1 ids");
+  if (!d_offsets || (n_ids && (!d_order || !d_keys || !d_slot))) return mvr::tok::bad(c, "null pointer");
+  if (!mvr::tok::aligned(d_offsets, 4) || !mvr::tok::aligned(d_order, 4) || !mvr::tok::aligned(d_keys, 4) || !mvr::tok::aligned(d_slot, 4))
+    return mvr::tok::bad(c, "an output is not aligned to its type");
+  uint64_t need = 0;
+  MVR_TRY(mvr_token_plan_bytes(n_ids, rows, &need));
+  MVR_TRY(mvr::tok::check_workspace(c, d_workspace, workspace_bytes, need));
+  mvr::DeviceScope dev_scope(c);
+  MVR_TRY(dev_scope.status);
+  cudaStream_t st = c->stream;
+  if (n_ids == 0) {
+    MVR_CUDA(c, cudaMemsetAsync(d_offsets, 0, (rows + 1) * 4, st));
+    return MVR_OK;
+  }
+  const mvr::tok::PlanArgs A = {d_ids,     id_bytes, (uint32_t)n_ids, (uint32_t)rows,
+                                d_offsets, d_order,  d_keys,          d_slot};
+  const mvr::tok::PlanSpace ws(n_ids, rows);
+  auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(d_workspace) + off); };
+  if (n_ids <= mvr::tok::kSmallMax) {
+    const mvr::tok::Digits D(rows, mvr::tok::kSmallBits);
+    MVR_TRY(mvr::tok::plan_small(c, A, D, at(ws.k0), at(ws.v0), at(ws.k1), at(ws.v1)));
+    if (D.passes == 1) return MVR_OK;  // the offsets came with the counts
+  } else {
+    const mvr::tok::Digits D(rows, mvr::tok::kTileBits);
+    MVR_TRY(mvr::tok::plan_tiles(c, A, D, at(ws.k0), at(ws.v0), at(ws.k1), at(ws.v1), at(ws.hist), at(ws.sums)));
+  }
+  MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_offsets_kernel, (unsigned)(rows / 256 + 1), 256, 0, st, A));
+  return MVR_OK;
+}
+
+}  // extern "C"

@@ -480,8 +480,9 @@ def _state(seed, n=1500):
                 scale=torch.rand(n, generator=g, device="cuda"), w=torch.rand(n, 2, generator=g, device="cuda"))
 
 
-def test_captured_graphs_replay_on_new_inputs():
-    states = [_state(40), _state(41)]
+@pytest.mark.parametrize("n", [1500, 70_001])
+def test_captured_graphs_replay_on_new_inputs(n):
+    states = [_state(40, n), _state(41, n)]
     for s in states:
         _pass(s)
     torch.cuda.synchronize()
@@ -492,7 +493,7 @@ def test_captured_graphs_replay_on_new_inputs():
             outs.append(_pass(s))
         graphs.append(gr)
     for k, (s, seed) in enumerate(zip(states, (50, 51))):
-        for name, v in _state(seed).items():
+        for name, v in _state(seed, n).items():
             s[name].copy_(v)
     # both graphs in flight at once, each on a stream of its own
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
