@@ -74,6 +74,9 @@ struct GradShape {
   uint32_t n, rows, dim;
   uint32_t lanes;     // L: lanes of a group, a power of two
   uint32_t per_group;  // Tg: places of a group, a multiple of 8
+  uint32_t tiles;      // blocks with places; those behind them fill rows without a token
+  uint32_t fill_lanes;  // lanes of a row there, a power of two
+  bool wide_plan;      // keys and order can be read four at a time
   uint64_t gs, ts, ds;  // row strides of grad, table, dtable
 };
 
@@ -92,28 +95,89 @@ struct GradArgs {
 };
 
 template <class O, int V>
-__device__ __forceinline__ void put_sum(O* p, const float (&sum)[V], int accumulate) {
+__device__ __forceinline__ void put_sum(O* p, const float (&sum)[V], float alpha, int accumulate) {
   Raw<O, V> r;
-  if (accumulate) {
-    float x[V];
+  float x[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = to_f32(p[v]) + sum[v];
-    r.set(x);
-  } else {
-    r.set(sum);
-  }
+  for (int v = 0; v < V; ++v) x[v] = accumulate ? fmaf(alpha, sum[v], to_f32(p[v])) : alpha * sum[v];
+  r.set(x);
   r.store(p);
+}
+
+// Zeros for the rows without a token: a warp looks at 32 rows at once.
+template <class O, int V>
+__device__ __forceinline__ void fill_empty_rows(const GradShape& S, const uint32_t* __restrict__ offsets,
+                                                O* __restrict__ dtable) {
+  const uint64_t block = (uint64_t)(blockIdx.x - S.tiles) * gridDim.y + blockIdx.y;
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t v0 = block * 256 + (threadIdx.x & ~31u);
+  const uint64_t v = v0 + lane;
+  const uint32_t empty = __ballot_sync(0xffffffffu, v < S.rows && offsets[v] == offsets[v + 1]);
+  const uint32_t chunks = S.dim / V, L = S.fill_lanes;
+  Raw<O, V> z;
+  z.zero();
+  for (uint32_t j = lane / L; j < 32; j += 32 / L)
+    if (empty >> j & 1)
+      for (uint32_t c = lane & (L - 1); c < chunks; c += L) z.store(dtable + (v0 + j) * S.ds + (uint64_t)c * V);
+}
+
+// Sums of U values over the L lanes of a group, all at once: while a lane has
+// several values, it gives half of them to the lane across and takes the other
+// half's, so they take U - 1 + log2(L / U) exchanges instead of U log2(L).
+template <int U>
+struct GroupSums {
+  uint32_t which = 0;  // x[k] has become the sum of value which + k, k < values
+  int values = U;      // one unless the group has fewer lanes than U
+  bool writes;         // whether this lane is the one to write them
+  __device__ __forceinline__ GroupSums(float (&x)[U], uint32_t L, uint32_t l) {
+    uint32_t o = L >> 1;
+#pragma unroll
+    for (int half = U >> 1; half > 0; half >>= 1) {
+      if (o == 0) continue;  // the same for all lanes
+      const bool up = l & o;
+#pragma unroll
+      for (int k = 0; k < half; ++k) {
+        const float give = up ? x[k] : x[k + half];
+        const float keep = up ? x[k + half] : x[k];
+        x[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+      which += up ? half : 0;
+      values = half;
+      o >>= 1;
+    }
+    writes = o == 0 || (l & (2 * o - 1)) == 0;
+    for (; o > 0; o >>= 1) x[0] += __shfl_xor_sync(0xffffffffu, x[0], o);
+  }
+};
+
+// Four consecutive words of the plan (places p0 .. p0 + 3 of a group's 8).
+__device__ __forceinline__ void load4(const uint32_t* p, bool wide, uint32_t (&x)[8], int at) {
+  if (wide) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p + at);
+    x[at] = v.x;
+    x[at + 1] = v.y;
+    x[at + 2] = v.z;
+    x[at + 3] = v.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[at + k] = p[at + k];
+  }
 }
 
 template <class T, class O, int V, bool DSCALE>
 __global__ void __launch_bounds__(256)
 lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   constexpr int NCH = chunks_per_lane<T, V>();
-  constexpr int U = DSCALE ? 4 : 8;  // rows in flight a lane
+  constexpr int U = 8;  // rows in flight a lane
   __shared__ float s_head[256 * NCH * V], s_tail[256 * NCH * V];
   __shared__ uint8_t s_hkind[256], s_has_tail[256];  // head: 0 none, 1 ends here, 2 goes on
-  __shared__ uint32_t s_hkey[256], s_tkey[256];
+  __shared__ uint32_t s_tkey[256];
+  grid_dependency_wait();
   const GradShape& S = A.s;
+  if (blockIdx.x >= S.tiles) {
+    fill_empty_rows<O, V>(S, A.offsets, A.dtable);
+    return;
+  }
   const uint32_t L = S.lanes, G = 256 / L;
   const uint32_t g = threadIdx.x / L, l = threadIdx.x & (L - 1);
   const uint32_t valid = min(A.offsets[S.rows], S.n);
@@ -142,10 +206,6 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
       for (int v = 0; v < V; ++v) acc[k][v] = 0.f;
   };
   clear();
-
-  bool started = a < b && (a == 0 || A.keys[a - 1] != A.keys[a]);
-  uint32_t cur = a < b ? A.keys[a] : S.rows;
-  uint32_t hkind = 0;
   auto stage = [&](float* where) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k)
@@ -156,67 +216,115 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
     if (key < S.rows)
 #pragma unroll
       for (int k = 0; k < NCH; ++k)
-        if (on[k]) put_sum(A.dtable + (uint64_t)key * S.ds + col[k], acc[k], A.accumulate);
+        if (on[k]) put_sum(A.dtable + (uint64_t)key * S.ds + col[k], acc[k], A.alpha, A.accumulate);
   };
 
-  const uint32_t steps = (S.per_group + U - 1) / U;  // the same for all lanes: shuffles inside
+  bool started = a < b && (a == 0 || A.keys[a - 1] != A.keys[a]);
+  uint32_t cur = a < b ? A.keys[a] : S.rows;
+  uint32_t hkind = 0;
+  Raw<T, V> trow[NCH];  // the table's row of `cur`
+  auto load_row = [&](Raw<T, V> (&r)[NCH], const T* base, uint64_t at, bool in) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      r[k].zero();
+      if (in && on[k]) r[k].load(base + at + col[k]);
+    }
+  };
+  if constexpr (DSCALE) load_row(trow, A.table, cur * S.ts, cur < S.rows);
+
+  const bool wide = S.wide_plan;
+  const uint32_t steps = S.per_group / U;  // the same for all lanes: exchanges inside
   for (uint32_t step = 0; step < steps; ++step) {
     const uint32_t p0 = a + step * U;
     if (__all_sync(0xffffffffu, p0 >= b)) break;
     uint32_t key[U], tok[U];
     float f[U];
-    Raw<T, V> row[U][NCH], trow[DSCALE ? U : 1][NCH];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = p0 + u < b;
-      key[u] = in ? A.keys[p0 + u] : S.rows;
-      tok[u] = in ? A.order[p0 + u] : S.n;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = tok[u] < S.n && key[u] < S.rows;
-      f[u] = in ? (A.scale ? A.alpha * A.scale[tok[u]] : A.alpha) : 0.f;
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        row[u][k].zero();
-        if (in && on[k]) row[u][k].load(A.grad + tok[u] * S.gs + col[k]);
-        if constexpr (DSCALE) {
-          trow[u][k].zero();
-          if (in && on[k]) trow[u][k].load(A.table + key[u] * S.ts + col[k]);
-        }
-      }
-    }
-    if constexpr (DSCALE) {
+    Raw<T, V> row[U][NCH];
+    if (p0 + U <= b) {
+      load4(A.keys + p0, wide, key, 0);
+      load4(A.keys + p0, wide, key, 4);
+      load4(A.order + p0, wide, tok, 0);
+      load4(A.order + p0, wide, tok, 4);
+    } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float dot = 0.f;
-#pragma unroll
-        for (int k = 0; k < NCH; ++k)
-#pragma unroll
-          for (int v = 0; v < V; ++v) dot = fmaf(row[u][k].get(v), trow[u][k].get(v), dot);
-        for (uint32_t o = L >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (l == 0 && tok[u] < S.n) A.dscale[tok[u]] = A.alpha * dot;
+        const bool in = p0 + u < b;
+        key[u] = in ? A.keys[p0 + u] : S.rows;
+        tok[u] = in ? A.order[p0 + u] : S.n;
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (p0 + u < b) {
-        if (key[u] != cur) {
-          if (started) {
-            write(cur);
-          } else {
-            stage(s_head);
-            hkind = 1;
-            if (l == 0) s_hkey[g] = cur;
-          }
-          started = true;
-          cur = key[u];
-          clear();
+      const bool in = tok[u] < S.n;
+      f[u] = in ? (A.scale ? A.scale[tok[u]] : 1.f) : 0.f;
+      load_row(row[u], A.grad, tok[u] * S.gs, in);
+    }
+    // bit u: place p0 + u begins a key
+    uint32_t begins = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p0 + u < b && key[u] != (u ? key[u - 1] : cur)) begins |= 1u << u;
+    float dot[U];
+    if constexpr (DSCALE) {
+      if (begins == 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          dot[u] = 0.f;
+#pragma unroll
+          for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) dot[u] = fmaf(row[u][k].get(v), trow[k].get(v), dot[u]);
+        }
+      } else {
+        Raw<T, V> other[U][NCH];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_row(other[u], A.table, key[u] * S.ts, key[u] < S.rows);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          dot[u] = 0.f;
+#pragma unroll
+          for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) dot[u] = fmaf(row[u][k].get(v), other[u][k].get(v), dot[u]);
         }
 #pragma unroll
-        for (int k = 0; k < NCH; ++k)
+        for (int k = 0; k < NCH; ++k) trow[k] = other[U - 1][k];  // of the last place's key
+      }
+    }
+    // the places up to the next key's first, then that key
+    for (uint32_t from = 0;;) {
+      const uint32_t rest = begins & ~((1u << from) - 1u);
+      const uint32_t to = rest ? __ffs(rest) - 1 : U;
 #pragma unroll
-          for (int v = 0; v < V; ++v) acc[k][v] = fmaf(f[u], row[u][k].get(v), acc[k][v]);
+      for (int u = 0; u < U; ++u)
+        if (u >= (int)from && u < (int)to) {
+#pragma unroll
+          for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[k][v] = fmaf(f[u], row[u][k].get(v), acc[k][v]);
+        }
+      if (!rest) break;
+      if (started) {
+        write(cur);
+      } else {
+        stage(s_head);
+        hkind = 1;
+      }
+      started = true;
+      clear();
+      cur = A.keys[p0 + to];
+      begins &= ~(1u << to);
+      from = to;
+    }
+    if constexpr (DSCALE) {
+      const GroupSums<U> sums(dot, L, l);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const uint32_t p = p0 + sums.which + k;
+        if (sums.writes && k < sums.values && p < b) {
+          const uint32_t t = A.order[p];
+          if (t < S.n) A.dscale[t] = A.alpha * dot[k];
+        }
       }
     }
   }
@@ -228,7 +336,6 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
     } else if (!started) {
       stage(s_head);
       hkind = ends ? 1 : 2;
-      if (l == 0) s_hkey[g] = cur;
     } else {
       stage(s_tail);
       has_tail = true;
@@ -244,10 +351,9 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   // a group that began a key which goes on adds what the next groups have of
   // it; the first group does the same for a key that began in an earlier block
   const bool from_before = g == 0 && s_hkind[0] != 0;
-#pragma unroll
+#pragma unroll 1
   for (int turn = 0; turn < 2; ++turn) {
     if (turn == 0 ? !from_before : !s_has_tail[g]) continue;
-    const uint32_t key = turn == 0 ? s_hkey[0] : s_tkey[g];
     const float* first = turn == 0 ? s_head : s_tail;
 #pragma unroll
     for (int k = 0; k < NCH; ++k)
@@ -262,7 +368,7 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
       open = s_hkind[q] == 2;
     }
     if (turn == 1 && !open) {
-      write(key);
+      write(s_tkey[g]);
     } else {
       float* out = A.part + ((uint64_t)blockIdx.x * 2 + (open ? 1 : 0)) * S.dim;
 #pragma unroll
@@ -274,41 +380,23 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   }
 }
 
-// Rows without a token become zeros (blocks from `joins` on), and block t <
-// joins sums the key that crosses the border of tiles t and t + 1 and has
-// crossed no earlier one: what it left behind the tiles, in their order, then
-// its end.
-template <class O, int V>
+// Block t sums the key that crosses the border of tiles t and t + 1 and has
+// crossed no earlier one: what it left behind the tiles, in their order (the
+// warps take every eighth), then its end.
+template <class O>
 __global__ void __launch_bounds__(256)
-lookup_grad_join_kernel(GradShape S, uint32_t tile, uint32_t joins, const uint32_t* __restrict__ offsets,
+lookup_grad_join_kernel(GradShape S, uint32_t tile, const uint32_t* __restrict__ offsets,
                         const uint32_t* __restrict__ keys, const float* __restrict__ part, O* __restrict__ dtable,
-                        int accumulate) {
-  if (blockIdx.x >= joins) {
-    if (accumulate) return;
-    const uint32_t chunks = S.dim / V;
-    const uint64_t total = (uint64_t)S.rows * chunks;
-    for (uint64_t e = (uint64_t)(blockIdx.x - joins) * 256 + threadIdx.x; e < total;
-         e += (uint64_t)(gridDim.x - joins) * 256) {
-      const uint32_t v = (uint32_t)(e / chunks), c = (uint32_t)(e - (uint64_t)v * chunks);
-      if (offsets[v] == offsets[v + 1]) {
-        Raw<O, V> z;
-        z.zero();
-        z.store(dtable + v * S.ds + c * V);
-      }
-    }
-    return;
-  }
-  const uint32_t valid = min(offsets[S.rows], S.n);
+                        float alpha, int accumulate) {
+  grid_dependency_wait();
   const uint64_t border = (uint64_t)(blockIdx.x + 1) * tile;
-  if (border >= valid) return;
-  const uint32_t key = keys[border];
-  if (key >= S.rows || keys[border - 1] != key) return;
-  const uint32_t first = offsets[key] / tile, last = (min(offsets[key + 1], valid) - 1) / tile;
+  const uint32_t key = keys[border], before = keys[border - 1];
+  if (key >= S.rows || before != key) return;
+  const uint32_t first = offsets[key] / tile, last = min((offsets[key + 1] - 1) / tile, S.tiles - 1);
   if (first != blockIdx.x) return;
   __shared__ float s_sum[256];
-  // 32 columns at a time, 8 warps over the tiles
   const uint32_t w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  for (uint32_t c0 = 0; c0 < S.dim; c0 += 32) {
+  for (uint32_t c0 = blockIdx.y * 32; c0 < S.dim; c0 += gridDim.y * 32) {
     const uint32_t c = c0 + l;
     float acc = 0.f;
     if (c < S.dim) {
@@ -321,8 +409,8 @@ lookup_grad_join_kernel(GradShape S, uint32_t tile, uint32_t joins, const uint32
 #pragma unroll
       for (int q = 1; q < 8; ++q) acc += s_sum[q * 32 + l];
       acc += part[(uint64_t)last * 2 * S.dim + c];
-      O* o = dtable + (uint64_t)key * S.ds + c;
-      *o = from_f32<O>(accumulate ? to_f32(*o) + acc : acc);
+      const float sum[1] = {acc};
+      put_sum<O, 1>(dtable + (uint64_t)key * S.ds + c, sum, alpha, accumulate);
     }
     __syncthreads();
   }
@@ -387,24 +475,24 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
              8ull * c->sm_count)
     S.per_group >>= 1;
   const uint32_t tile = groups * S.per_group;
-  const uint32_t tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
-  if (tiles) {
-    if (A.dscale && slabs == 1)
-      lookup_grad_tile_kernel<T, O, V, true><<<dim3(tiles, slabs), 256, 0, st>>>(A);
-    else
-      lookup_grad_tile_kernel<T, O, V, false><<<dim3(tiles, slabs), 256, 0, st>>>(A);
-    if (A.dscale && slabs > 1) {  // a row's parts lie in several blocks
-      const uint32_t L = lanes_of(c, S.n, chunks);
-      lookup_dscale_kernel<T, V><<<blocks_of(S.n, 256 / L), 256, 0, st>>>(
-          L, chunks, A.grad, S.gs, S.n, S.rows, A.keys, slot, A.alpha, A.table, S.ts, A.dscale);
-    }
+  S.tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
+  S.wide_plan = aligned(A.keys, 16) && aligned(A.order, 16);
+  S.fill_lanes = std::min(32u, pow2_ceil(chunks));
+  const uint32_t fill = A.accumulate ? 0 : (uint32_t)(((S.rows + 255ull) / 256 + slabs - 1) / slabs);
+  if (S.tiles + fill == 0) return MVR_OK;
+  const bool with_dscale = A.dscale && slabs == 1;
+  const auto kernel = with_dscale ? lookup_grad_tile_kernel<T, O, V, true> : lookup_grad_tile_kernel<T, O, V, false>;
+  MVR_CUDA(c, launch_pdl(kernel, dim3(S.tiles + fill, slabs), 256, 0, st, A));
+  if (S.tiles > 1)  // 32 columns a block while the grid stays small: most blocks have nothing to join
+    MVR_CUDA(c, launch_pdl(lookup_grad_join_kernel<O>,
+                           dim3(S.tiles - 1, std::max(1u, std::min((S.dim + 31) / 32, 32768u / S.tiles))), 256, 0, st, S, tile, A.offsets, A.keys, A.part,
+                           A.dtable, A.alpha, A.accumulate));
+  if (A.dscale && S.tiles && !with_dscale) {  // a row's parts lie in several blocks
+    const uint32_t L = lanes_of(c, S.n, chunks);
+    lookup_dscale_kernel<T, V><<<blocks_of(S.n, 256 / L), 256, 0, st>>>(L, chunks, A.grad, S.gs, S.n, S.rows, A.keys,
+                                                                       slot, A.alpha, A.table, S.ts, A.dscale);
+    MVR_CUDA(c, cudaGetLastError());
   }
-  const uint32_t joins = tiles ? tiles - 1 : 0;
-  const uint64_t fill = A.accumulate ? 0 : std::min<uint64_t>(((uint64_t)S.rows * chunks + 255) / 256, 8ull * c->sm_count);
-  if (joins + fill)
-    lookup_grad_join_kernel<O, V><<<(unsigned)(joins + fill), 256, 0, st>>>(S, tile, joins, A.offsets, A.keys, A.part,
-                                                                           A.dtable, A.accumulate);
-  MVR_CUDA(c, cudaGetLastError());
   return MVR_OK;
 }
 
@@ -490,7 +578,7 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
       return mvr::tok::by_vec<T>(w, [&](auto vec) {
         constexpr int V = decltype(vec)::value;
         mvr::tok::GradArgs<T, O, V> A;
-        A.s = {n, v, dim, 0, 0, grad_stride, table_stride, dtable_stride};
+        A.s = {n, v, dim, 0, 0, 0, 0, false, grad_stride, table_stride, dtable_stride};
         A.grad = (const T*)d_grad;
         A.offsets = d_offsets;
         A.order = d_order;

@@ -2,6 +2,8 @@
 // the grouping of rows read. include/mvr.h states what it gives.
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "token_ops.cuh"
 
 namespace cg = cooperative_groups;
@@ -18,8 +20,8 @@ namespace {
 
 constexpr uint32_t kSmallThreads = 1024, kSmallRounds = 8, kSmallBlocks = 8;
 constexpr uint32_t kSmallMax = kSmallThreads * kSmallRounds * kSmallBlocks;  // 65,536 pairs
-constexpr int kSmallBits = 9;                                                // of a digit
-constexpr uint32_t kTileThreads = 256, kTileRounds = 16, kTile = kTileThreads * kTileRounds;
+constexpr int kSmallBits = 11;                                               // of a digit
+constexpr uint32_t kTileThreads = 512, kTileRounds = 8, kTile = kTileThreads * kTileRounds;
 constexpr int kTileBits = 10;
 
 struct PlanArgs {
@@ -29,31 +31,53 @@ struct PlanArgs {
   uint32_t *offsets, *order, *keys, *slot;
 };
 
-// Equal digits among the warp's lanes: how many are below this lane, and
-// whether it is the first.
+// Where a pass reads its keys: the ids (4 or 8 bytes) or the last pass's.
+template <class I>
+__device__ __forceinline__ uint32_t key_at(const void* src, uint64_t e, uint32_t rows) {
+  if constexpr (std::is_same_v<I, void>) {
+    return __ldcg(static_cast<const uint32_t*>(src) + e);
+  } else {
+    const I id = static_cast<const I*>(src)[e];
+    return id < rows ? (uint32_t)id : rows;
+  }
+}
+
+// Equal digits among the warp's lanes that are `in`: how many are below this
+// lane, and how many there are. (One vote a bit of the digit measured slower.)
 struct Peers {
   uint32_t below, count;
-  __device__ __forceinline__ explicit Peers(uint32_t digit) {
-    const uint32_t m = __match_any_sync(0xffffffffu, digit);
+  __device__ __forceinline__ Peers(uint32_t digit, bool in) {
+    const uint32_t m = __match_any_sync(0xffffffffu, in ? digit : ~(threadIdx.x & 31));
     below = __popc(m & lanemask_lt());
     count = __popc(m);
   }
 };
 
-// Exclusive prefix sums of s[0 .. R), R a power of two up to 4 a thread, by all
-// `threads` threads of the block (a multiple of 32, at most 1024). w: one value
-// a warp.
+// A digit's counts in the warps' rows of s, R apart, become those of the warps
+// before; their sum.
+__device__ __forceinline__ uint32_t warps_prefix(uint16_t* s, uint32_t R, uint32_t warps) {
+  uint32_t run = 0;
+#pragma unroll 4
+  for (uint32_t q = 0; q < warps; ++q) {
+    const uint32_t x = s[q * R];
+    s[q * R] = (uint16_t)run;
+    run += x;
+  }
+  return run;
+}
+
+// Exclusive prefix sums of s[0 .. R) by all `threads` threads of the block (a
+// multiple of 32, at most 1024). w: one value a warp. These kernels run through
+// their code once, so its length is time: loops are kept as loops.
 __device__ __forceinline__ void block_prefix(uint32_t* s, uint32_t R, uint32_t threads, uint32_t* w) {
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const uint32_t per = R <= threads ? 1 : R / threads;
-  uint32_t v[4], sum = 0;
-#pragma unroll
-  for (uint32_t k = 0; k < 4; ++k) {
-    v[k] = k < per && t * per + k < R ? s[t * per + k] : 0;
-    sum += v[k];
-  }
+  const uint32_t per = (R + threads - 1) / threads;
+  const uint32_t lo = min(R, t * per), hi = min(R, lo + per);
+  uint32_t sum = 0;
+#pragma unroll 1
+  for (uint32_t k = lo; k < hi; ++k) sum += s[k];
   uint32_t run = sum;
-#pragma unroll
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t x = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= (uint32_t)o) run += x;
@@ -62,7 +86,7 @@ __device__ __forceinline__ void block_prefix(uint32_t* s, uint32_t R, uint32_t t
   __syncthreads();
   if (warp == 0) {
     uint32_t x = lane < threads / 32 ? w[lane] : 0;
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= (uint32_t)o) x += y;
@@ -71,90 +95,87 @@ __device__ __forceinline__ void block_prefix(uint32_t* s, uint32_t R, uint32_t t
   }
   __syncthreads();
   run += (warp ? w[warp - 1] : 0) - sum;
-#pragma unroll
-  for (uint32_t k = 0; k < 4; ++k)
-    if (k < per && t * per + k < R) {
-      s[t * per + k] = run;
-      run += v[k];
-    }
+#pragma unroll 1
+  for (uint32_t k = lo; k < hi; ++k) {
+    const uint32_t x = s[k];
+    s[k] = run;
+    run += x;
+  }
   __syncthreads();
 }
 
-// All passes over at most kSmallMax pairs by one cluster. Block c has the
-// pairs [c * chunk, (c + 1) * chunk), a warp 32 x rounds of them in order, and
-// the blocks read one another's digit counts from shared memory. With one
-// pass the digits are the keys, and their prefix sums the offsets.
+// All passes over at most kSmallMax pairs by one cluster. A warp has 32 x
+// rounds pairs in order, the blocks read one another's digit counts from shared
+// memory. With one pass the digits are the keys, and their prefix sums the
+// offsets.
+template <class I>
 __global__ void __launch_bounds__(kSmallThreads)
 plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint32_t* k0, uint32_t* v0, uint32_t* k1,
                   uint32_t* v1) {
-  __shared__ uint16_t s_count[32][1 << kSmallBits];  // a warp's pairs of a digit; then those of the warps before
-  __shared__ uint32_t s_total[1 << kSmallBits], s_base[1 << kSmallBits], s_warp[32];
+  extern __shared__ uint32_t smem[];
+  __shared__ uint32_t s_warp[32];
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t rank = cluster.block_rank(), blocks = cluster.num_blocks();
+  const uint32_t threads = blockDim.x, warps = threads / 32;
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint32_t R = 1u << digit_bits;
-  const uint32_t first = rank * (rounds * kSmallThreads) + warp * (rounds * 32) + lane;
+  uint32_t* s_total = smem;       // [R] the block's pairs of a digit
+  uint32_t* s_base = s_total + R;  // [R] first place of the digit
+  uint32_t* s_before = s_base + R;  // [R] its pairs in the blocks before
+  uint16_t* s_count = reinterpret_cast<uint16_t*>(s_before + R);  // [warps][R] a warp's; then those of the warps before
+  uint16_t* mine = s_count + warp * R;
+  const uint32_t first = rank * (rounds * threads) + warp * (rounds * 32) + lane;
   const uint32_t *kin = nullptr, *vin = nullptr;
   uint32_t *kout = k0, *vout = v0;
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
     const bool last = pass + 1 == passes;
-    for (uint32_t e = t; e < 32 * R; e += kSmallThreads) s_count[e >> digit_bits][e & (R - 1)] = 0;
     uint32_t key[kSmallRounds], val[kSmallRounds], place[kSmallRounds];
 #pragma unroll
     for (uint32_t j = 0; j < kSmallRounds; ++j) {
+      if (j >= rounds) break;
       const uint32_t e = first + j * 32;
       key[j] = val[j] = 0;
-      if (j < rounds && e < A.n) {
-        key[j] = pass ? __ldcg(kin + e) : row_of(A.ids, A.id_bytes, e, A.rows);
+      if (e < A.n) {
+        key[j] = pass ? key_at<void>(kin, e, 0) : key_at<I>(A.ids, e, A.rows);
         val[j] = pass ? __ldcg(vin + e) : e;
       }
     }
+    for (uint32_t e = t; e < warps * R / 2; e += threads) reinterpret_cast<uint32_t*>(s_count)[e] = 0;
     __syncthreads();
 #pragma unroll
     for (uint32_t j = 0; j < kSmallRounds; ++j) {
       if (j >= rounds) break;
       const bool in = first + j * 32 < A.n;
       const uint32_t d = (key[j] >> shift) & (R - 1);
-      const Peers p(in ? d : R + lane);
-      if (in) place[j] = s_count[warp][d] + p.below;
+      const Peers p(d, in);
+      if (in) place[j] = mine[d] + p.below;
       __syncwarp();
-      if (in && p.below == 0) s_count[warp][d] += (uint16_t)p.count;
+      if (in && p.below == 0) mine[d] += (uint16_t)p.count;
       __syncwarp();
     }
     __syncthreads();
-    if (t < R) {
-      uint32_t run = 0;
-#pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        const uint32_t x = s_count[q][t];
-        s_count[q][t] = (uint16_t)run;
-        run += x;
-      }
-      s_total[t] = run;
-    }
+    for (uint32_t d = t; d < R; d += threads) s_total[d] = warps_prefix(s_count + d, R, warps);
     cluster.sync();
-    uint32_t before = 0, all = 0;
-    if (t < R) {
+    for (uint32_t d = t; d < R; d += threads) {
+      uint32_t before = 0, all = 0;
       for (uint32_t q = 0; q < blocks; ++q) {
-        const uint32_t x = *cluster.map_shared_rank(&s_total[t], q);
+        const uint32_t x = *cluster.map_shared_rank(s_total + d, q);
         if (q < rank) before += x;
         all += x;
       }
-      s_base[t] = all;
+      s_base[d] = all;
+      s_before[d] = before;
     }
     __syncthreads();
-    block_prefix(s_base, R, kSmallThreads, s_warp);
-    if (t < R) {
-      if (passes == 1 && rank == 0 && t <= A.rows) A.offsets[t] = s_base[t];
-      s_base[t] += before;
-    }
-    __syncthreads();
+    block_prefix(s_base, R, threads, s_warp);
+    if (passes == 1 && rank == 0)
+      for (uint32_t d = t; d <= A.rows; d += threads) A.offsets[d] = s_base[d];
 #pragma unroll
     for (uint32_t j = 0; j < kSmallRounds; ++j) {
       if (j >= rounds || first + j * 32 >= A.n) break;
       const uint32_t d = (key[j] >> shift) & (R - 1);
-      const uint32_t pos = s_base[d] + s_count[warp][d] + place[j];
+      const uint32_t pos = s_base[d] + s_before[d] + mine[d] + place[j];
       if (last) {
         A.keys[pos] = key[j];
         A.order[pos] = val[j];
@@ -173,8 +194,9 @@ plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint3
 }
 
 // Pairs of each digit in a tile: hist[digit][tile].
+template <class I>
 __global__ void __launch_bounds__(kTileThreads)
-plan_hist_kernel(PlanArgs A, const uint32_t* __restrict__ kin, int shift, uint32_t R, uint32_t tiles,
+plan_hist_kernel(const void* __restrict__ src, uint32_t n, uint32_t rows, int shift, uint32_t R, uint32_t tiles,
                  uint32_t* __restrict__ hist) {
   __shared__ uint32_t s_count[1 << kTileBits];
   grid_dependency_wait();
@@ -182,14 +204,15 @@ plan_hist_kernel(PlanArgs A, const uint32_t* __restrict__ kin, int shift, uint32
   for (uint32_t d = t; d < R; d += kTileThreads) s_count[d] = 0;
   __syncthreads();
   const uint64_t first = (uint64_t)blockIdx.x * kTile + t;
+  uint32_t key[kTileRounds];
 #pragma unroll
   for (uint32_t j = 0; j < kTileRounds; ++j) {
     const uint64_t e = first + j * kTileThreads;
-    if (e < A.n) {
-      const uint32_t key = kin ? kin[e] : row_of(A.ids, A.id_bytes, e, A.rows);
-      atomicAdd(&s_count[(key >> shift) & (R - 1)], 1u);
-    }
+    key[j] = e < n ? key_at<I>(src, e, rows) : ~0u;
   }
+#pragma unroll
+  for (uint32_t j = 0; j < kTileRounds; ++j)
+    if (first + j * kTileThreads < n) atomicAdd(&s_count[(key[j] >> shift) & (R - 1)], 1u);
   __syncthreads();
   for (uint32_t d = t; d < R; d += kTileThreads) hist[(uint64_t)d * tiles + blockIdx.x] = s_count[d];
 }
@@ -223,12 +246,13 @@ plan_scan_kernel(uint32_t tiles, uint32_t* __restrict__ hist, uint32_t* __restri
 
 // A tile's pairs, sorted by digit in shared memory first so that each digit's
 // run is written in one piece.
-template <bool LAST>
+template <class I, bool LAST>
 __global__ void __launch_bounds__(kTileThreads)
-plan_scatter_kernel(PlanArgs A, const uint32_t* __restrict__ kin, const uint32_t* __restrict__ vin, int shift,
-                    uint32_t R, uint32_t tiles, const uint32_t* __restrict__ hist,
+plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __restrict__ vin, int shift,
+                    int bits, uint32_t tiles, const uint32_t* __restrict__ hist,
                     const uint32_t* __restrict__ total, uint32_t* __restrict__ kout, uint32_t* __restrict__ vout) {
   constexpr uint32_t kWarps = kTileThreads / 32;
+  const uint32_t R = 1u << bits;
   extern __shared__ uint32_t smem[];
   uint32_t* s_key = smem;              // [kTile]
   uint32_t* s_val = s_key + kTile;     // [kTile]
@@ -249,8 +273,8 @@ plan_scatter_kernel(PlanArgs A, const uint32_t* __restrict__ kin, const uint32_t
     const uint32_t q = first + j * 32;
     key[j] = val[j] = 0;
     if (q < in_tile) {
-      key[j] = kin ? kin[tile0 + q] : row_of(A.ids, A.id_bytes, tile0 + q, A.rows);
-      val[j] = vin ? vin[tile0 + q] : (uint32_t)(tile0 + q);
+      key[j] = key_at<I>(src, tile0 + q, A.rows);
+      val[j] = std::is_same_v<I, void> ? __ldcg(vin + tile0 + q) : (uint32_t)(tile0 + q);
     }
   }
   __syncthreads();
@@ -260,23 +284,14 @@ plan_scatter_kernel(PlanArgs A, const uint32_t* __restrict__ kin, const uint32_t
   for (uint32_t j = 0; j < kTileRounds; ++j) {
     const bool in = first + j * 32 < in_tile;
     const uint32_t d = (key[j] >> shift) & (R - 1);
-    const Peers p(in ? d : R + lane);
+    const Peers p(d, in);
     if (in) place[j] = mine[d] + p.below;
     __syncwarp();
     if (in && p.below == 0) mine[d] += (uint16_t)p.count;
     __syncwarp();
   }
   __syncthreads();
-  for (uint32_t d = t; d < R; d += kTileThreads) {
-    uint32_t run = 0;
-#pragma unroll
-    for (uint32_t q = 0; q < kWarps; ++q) {
-      const uint32_t x = s_count[q * R + d];
-      s_count[q * R + d] = (uint16_t)run;
-      run += x;
-    }
-    s_start[d] = run;
-  }
+  for (uint32_t d = t; d < R; d += kTileThreads) s_start[d] = warps_prefix(s_count + d, R, kWarps);
   __syncthreads();
   block_prefix(s_start, R, kTileThreads, s_warp);
   for (uint32_t d = t; d < R; d += kTileThreads)
@@ -308,7 +323,8 @@ plan_scatter_kernel(PlanArgs A, const uint32_t* __restrict__ kin, const uint32_t
   }
 }
 
-// offsets[v] = first place whose key is >= v, by bisection.
+// offsets[v] = first place whose key is >= v, for rows far more than places:
+// by bisection, a thread a row.
 __global__ void __launch_bounds__(256) plan_offsets_kernel(PlanArgs A) {
   grid_dependency_wait();
   const uint32_t v = blockIdx.x * 256u + threadIdx.x;
@@ -322,6 +338,44 @@ __global__ void __launch_bounds__(256) plan_offsets_kernel(PlanArgs A) {
       hi = mid;
   }
   A.offsets[v] = lo;
+}
+
+// The same for rows of the places' number: place p (n included) fills the rows
+// behind the key before it up to its own. Gaps up to kOwnFill are filled by
+// their thread, up to kWarpFill by its warp, longer ones by the block.
+constexpr uint32_t kOwnFill = 4, kWarpFill = 1024;
+__global__ void __launch_bounds__(256) plan_borders_kernel(PlanArgs A) {
+  __shared__ uint32_t s_gaps, s_lo[256], s_hi[256], s_place[256];
+  grid_dependency_wait();
+  if (threadIdx.x == 0) s_gaps = 0;
+  __syncthreads();
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  uint32_t lo = 0, hi = 0;  // rows to fill
+  if (p <= A.n) {
+    lo = p ? A.keys[p - 1] + 1 : 0;
+    hi = p < A.n ? A.keys[p] + 1 : A.rows + 1;
+  }
+  const uint32_t gap = lo < hi ? hi - lo : 0;
+  if (gap <= kOwnFill) {
+    for (uint32_t v = lo; v < lo + gap; ++v) A.offsets[v] = (uint32_t)p;
+  } else if (gap > kWarpFill) {
+    const uint32_t g = atomicAdd(&s_gaps, 1u);
+    s_lo[g] = lo;
+    s_hi[g] = hi;
+    s_place[g] = (uint32_t)p;
+  }
+  uint32_t todo = __ballot_sync(0xffffffffu, gap > kOwnFill && gap <= kWarpFill);
+  while (todo) {
+    const int l = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const uint32_t from = __shfl_sync(0xffffffffu, lo, l), to = __shfl_sync(0xffffffffu, hi, l);
+    const uint32_t place = __shfl_sync(0xffffffffu, (uint32_t)p, l);
+    for (uint32_t v = from + lane; v < to; v += 32) A.offsets[v] = place;
+  }
+  __syncthreads();
+  for (uint32_t g = 0; g < s_gaps; ++g)
+    for (uint64_t v = (uint64_t)s_lo[g] + threadIdx.x; v < s_hi[g]; v += 256) A.offsets[v] = s_place[g];
 }
 
 struct Digits {
@@ -356,14 +410,22 @@ struct PlanSpace {
   }
 };
 
+template <class I>
 int plan_small(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_t* v0, uint32_t* k1, uint32_t* v1) {
-  // 2048 pairs a block and more before another block joins
+  // another block joins for every 2048 pairs; a block has the warps that its
+  // pairs fill, and some more for the prefix sums of many digits
+  const uint32_t R = 1u << D.bits;
   const uint32_t blocks = std::min(kSmallBlocks, pow2_ceil((A.n + 2047) / 2048));
   const uint32_t chunk = (A.n + blocks - 1) / blocks;
-  const uint32_t rounds = (chunk + kSmallThreads - 1) / kSmallThreads;
+  const uint32_t threads =
+      std::min(kSmallThreads, std::max({(chunk + 31) / 32 * 32, std::min(R, 256u), 64u}));
+  const uint32_t rounds = (chunk + threads - 1) / threads;
+  const size_t smem = 3 * R * 4 + (size_t)threads / 32 * R * 2;
+  MVR_CUDA(c, raise_smem_limit((const void*)plan_small_kernel<I>, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = blocks;
-  cfg.blockDim = kSmallThreads;
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = c->stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -371,30 +433,35 @@ int plan_small(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  MVR_CUDA(c, cudaLaunchKernelEx(&cfg, plan_small_kernel, A, rounds, D.bits, D.passes, k0, v0, k1, v1));
+  MVR_CUDA(c, cudaLaunchKernelEx(&cfg, plan_small_kernel<I>, A, rounds, D.bits, D.passes, k0, v0, k1, v1));
+  return MVR_OK;
+}
+
+// One pass over the tiles; I: what it reads its keys from.
+template <class I>
+int plan_pass(Ctx* c, const PlanArgs& A, const void* kin, const uint32_t* vin, int shift, int bits, bool last,
+              uint32_t* kout, uint32_t* vout, uint32_t* hist, uint32_t* sums) {
+  cudaStream_t st = c->stream;
+  const uint32_t tiles = (uint32_t)((A.n + (kTile - 1ull)) / kTile), R = 1u << bits;
+  const size_t smem = (2 * kTile + 2 * R) * 4 + kTileThreads / 32 * R * 2;
+  MVR_CUDA(c, launch_pdl(plan_hist_kernel<I>, tiles, kTileThreads, 0, st, kin, A.n, A.rows, shift, R, tiles, hist));
+  MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
+  const auto scatter = last ? plan_scatter_kernel<I, true> : plan_scatter_kernel<I, false>;
+  MVR_CUDA(c, raise_smem_limit((const void*)scatter, smem));
+  MVR_CUDA(c, launch_pdl(scatter, tiles, kTileThreads, smem, st, A, kin, vin, shift, bits, tiles, hist, sums, kout, vout));
   return MVR_OK;
 }
 
 int plan_tiles(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_t* v0, uint32_t* k1, uint32_t* v1,
                uint32_t* hist, uint32_t* sums) {
-  cudaStream_t st = c->stream;
-  const uint32_t tiles = (A.n + (kTile - 1ull)) / kTile, R = 1u << D.bits;
-  const size_t smem = (2 * kTile + 2 * R) * 4 + kTileThreads / 32 * R * 2;
-  MVR_CUDA(c, raise_smem_limit((const void*)plan_scatter_kernel<true>, smem));
-  MVR_CUDA(c, raise_smem_limit((const void*)plan_scatter_kernel<false>, smem));
-  const uint32_t *kin = nullptr, *vin = nullptr;
-  uint32_t *kout = k0, *vout = v0;
-  for (int pass = 0; pass < D.passes; ++pass) {
-    const int shift = pass * D.bits;
-    MVR_CUDA(c, launch_pdl(plan_hist_kernel, tiles, kTileThreads, 0, st, A, kin, shift, R, tiles, hist));
-    MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
-    const auto scatter = pass + 1 == D.passes ? plan_scatter_kernel<true> : plan_scatter_kernel<false>;
-    MVR_CUDA(c, launch_pdl(scatter, tiles, kTileThreads, smem, st, A, kin, vin, shift, R, tiles, hist, sums, kout,
-                           vout));
-    kin = kout;
-    vin = vout;
-    kout = kout == k0 ? k1 : k0;
-    vout = vout == v0 ? v1 : v0;
+  if (A.id_bytes == 8)
+    MVR_TRY(plan_pass<uint64_t>(c, A, A.ids, nullptr, 0, D.bits, D.passes == 1, k0, v0, hist, sums));
+  else
+    MVR_TRY(plan_pass<uint32_t>(c, A, A.ids, nullptr, 0, D.bits, D.passes == 1, k0, v0, hist, sums));
+  for (int pass = 1; pass < D.passes; ++pass) {
+    MVR_TRY(plan_pass<void>(c, A, k0, v0, pass * D.bits, D.bits, pass + 1 == D.passes, k1, v1, hist, sums));
+    std::swap(k0, k1);
+    std::swap(v0, v1);
   }
   return MVR_OK;
 }
@@ -439,13 +506,19 @@ int mvr_token_plan_device(mvr_ctx* h, const void* d_ids, int id_bytes, uint64_t 
   auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(d_workspace) + off); };
   if (n_ids <= mvr::tok::kSmallMax) {
     const mvr::tok::Digits D(rows, mvr::tok::kSmallBits);
-    MVR_TRY(mvr::tok::plan_small(c, A, D, at(ws.k0), at(ws.v0), at(ws.k1), at(ws.v1)));
+    const auto small = id_bytes == 8 ? mvr::tok::plan_small<uint64_t> : mvr::tok::plan_small<uint32_t>;
+    MVR_TRY(small(c, A, D, at(ws.k0), at(ws.v0), at(ws.k1), at(ws.v1)));
     if (D.passes == 1) return MVR_OK;  // the offsets came with the counts
   } else {
     const mvr::tok::Digits D(rows, mvr::tok::kTileBits);
     MVR_TRY(mvr::tok::plan_tiles(c, A, D, at(ws.k0), at(ws.v0), at(ws.k1), at(ws.v1), at(ws.hist), at(ws.sums)));
   }
-  MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_offsets_kernel, (unsigned)(rows / 256 + 1), 256, 0, st, A));
+  // Walking the places costs one read each, a search some twenty dependent ones
+  // a row: the walk is for rows that do not outnumber the places by far.
+  if (rows <= 8 * n_ids)
+    MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_borders_kernel, (unsigned)(n_ids / 256 + 1), 256, 0, st, A));
+  else
+    MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_offsets_kernel, (unsigned)(rows / 256 + 1), 256, 0, st, A));
   return MVR_OK;
 }
 
