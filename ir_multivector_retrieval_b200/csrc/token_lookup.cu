@@ -13,26 +13,26 @@ namespace {
 // so that a warp writes one run of memory whatever the row length; four of
 // them a thread, the block's stride apart, when there is work for all SMs.
 
-template <class T, int V, int UR>
+template <class T, class I, int V, int UR, bool SCALE>
 __global__ void __launch_bounds__(256)
-lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, const void* __restrict__ ids,
-              int id_bytes, const float* __restrict__ scale, float alpha, T* __restrict__ out, uint64_t os) {
+lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, const I* __restrict__ ids,
+              const float* __restrict__ scale, float alpha, T* __restrict__ out, uint64_t os) {
   const FlatBlock<UR> B(F);
   uint64_t i[UR];
   uint32_t c[UR], r[UR];
   float f[UR];
+  bool in[UR];
   Raw<T, V> x[UR];
+  // each loop is one wait for memory
 #pragma unroll
   for (int j = 0; j < UR; ++j) {
-    r[j] = rows;
-    f[j] = alpha;
-    if (B.at(j, &i[j], &c[j])) {
-      r[j] = row_of(ids, id_bytes, i[j], rows);
-      if (scale) f[j] = alpha * scale[i[j]];
-    } else {
-      i[j] = ~0ull;
-    }
+    in[j] = B.at(j, &i[j], &c[j]);
+    if (!in[j]) i[j] = c[j] = 0;  // read, not written
   }
+#pragma unroll
+  for (int j = 0; j < UR; ++j) r[j] = row_of<I>(ids, i[j], rows);
+#pragma unroll
+  for (int j = 0; j < UR; ++j) f[j] = SCALE ? alpha * scale[i[j]] : alpha;
 #pragma unroll
   for (int j = 0; j < UR; ++j) {
     x[j].zero();
@@ -40,7 +40,7 @@ lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, c
   }
 #pragma unroll
   for (int j = 0; j < UR; ++j) {
-    if (i[j] == ~0ull) continue;
+    if (!in[j]) continue;
     if (r[j] < rows) {
       float y[V];
 #pragma unroll
@@ -49,6 +49,18 @@ lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, c
     }
     x[j].store(out + i[j] * os + (uint64_t)c[j] * V);
   }
+}
+
+template <class T, class I, int V>
+int lookup_run(Ctx* c, const Flat& F, const void* table, uint64_t rows, uint64_t ts, const void* ids,
+               const float* scale, float alpha, void* out, uint64_t os) {
+  const bool four = many(c, F);
+  const auto kernel = scale ? (four ? lookup_kernel<T, I, V, 4, true> : lookup_kernel<T, I, V, 1, true>)
+                            : (four ? lookup_kernel<T, I, V, 4, false> : lookup_kernel<T, I, V, 1, false>);
+  kernel<<<blocks_of(F.total, four ? 1024 : 256), 256, 0, c->stream>>>(
+      F, (const T*)table, (uint32_t)rows, ts, (const I*)ids, scale, alpha, (T*)out, os);
+  MVR_CUDA(c, cudaGetLastError());
+  return MVR_OK;
 }
 
 // ---- lookup gradients ------------------------------------------------------
@@ -73,10 +85,9 @@ constexpr int chunks_per_lane() {
 struct GradShape {
   uint32_t n, rows, dim;
   uint32_t lanes;     // L: lanes of a group, a power of two
-  uint32_t per_group;  // Tg: places of a group, a multiple of 8
+  uint32_t per_group;  // Tg: places of a group
   uint32_t tiles;      // blocks with places; those behind them fill rows without a token
   uint32_t fill_lanes;  // lanes of a row there, a power of two
-  bool wide_plan;      // keys and order can be read four at a time
   uint64_t gs, ts, ds;  // row strides of grad, table, dtable
 };
 
@@ -148,27 +159,35 @@ struct GroupSums {
     writes = o == 0 || (l & (2 * o - 1)) == 0;
     for (; o > 0; o >>= 1) x[0] += __shfl_xor_sync(0xffffffffu, x[0], o);
   }
+  static __device__ __forceinline__ float at(const float (&x)[U], int k) {
+    float r = x[0];
+#pragma unroll
+    for (int q = 1; q < U; ++q) r = k == q ? x[q] : r;
+    return r;
+  }
 };
 
-// Four consecutive words of the plan (places p0 .. p0 + 3 of a group's 8).
-__device__ __forceinline__ void load4(const uint32_t* p, bool wide, uint32_t (&x)[8], int at) {
-  if (wide) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p + at);
-    x[at] = v.x;
-    x[at + 1] = v.y;
-    x[at + 2] = v.z;
-    x[at + 3] = v.w;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[at + k] = p[at + k];
-  }
+// Places of a tile whose plan entries a block keeps in shared memory.
+constexpr uint32_t kMaxTile = 2048;
+constexpr int kFlight = 4;  // rows a lane takes at once, and as many on their way
+
+// Bytes of a row's chunks in a lane.
+template <class T, int V>
+constexpr int lane_bytes() {
+  return chunks_per_lane<T, V>() * (int)sizeof(T) * V;
+}
+template <class T, int V>
+size_t grad_smem(uint32_t tile) {
+  return (size_t)2 * kFlight * lane_bytes<T, V>() * 256 + (size_t)tile * 12;
 }
 
 template <class T, class O, int V, bool DSCALE>
 __global__ void __launch_bounds__(256)
 lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   constexpr int NCH = chunks_per_lane<T, V>();
-  constexpr int U = 8;  // rows in flight a lane
+  constexpr int U = kFlight;
+  constexpr uint32_t kRing = 2u * U * lane_bytes<T, V>() * 256;
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float s_head[256 * NCH * V], s_tail[256 * NCH * V];
   __shared__ uint8_t s_hkind[256], s_has_tail[256];  // head: 0 none, 1 ends here, 2 goes on
   __shared__ uint32_t s_tkey[256];
@@ -189,8 +208,40 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
       if (A.order[p] < S.n) A.dscale[A.order[p]] = 0.f;
   }
   if (tile0 >= valid) return;
-  const uint32_t a = (uint32_t)min((uint64_t)valid, tile0 + (uint64_t)g * S.per_group);
-  const uint32_t b = (uint32_t)min((uint64_t)valid, tile0 + (uint64_t)(g + 1) * S.per_group);
+  // the tile's plan: keys, tokens, scales
+  uint32_t* s_key = reinterpret_cast<uint32_t*>(smem + kRing);
+  uint32_t* s_tok = s_key + tile;
+  float* s_scale = reinterpret_cast<float*>(s_tok + tile);
+  const uint32_t here = (uint32_t)min((uint64_t)tile, valid - tile0);
+  for (uint32_t e0 = 0; e0 < here; e0 += 1024) {  // four a thread at once: each loop is one wait for memory
+    uint32_t tok[4], key[4];
+    float f[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t e = e0 + q * 256 + threadIdx.x;
+      tok[q] = e < here ? A.order[tile0 + e] : 0;
+      key[q] = e < here ? A.keys[tile0 + e] : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (tok[q] >= S.n) tok[q] = 0;  // in bounds whatever the plan holds
+      f[q] = A.scale ? A.scale[tok[q]] : 1.f;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t e = e0 + q * 256 + threadIdx.x;
+      if (e < here) {
+        s_key[e] = key[q];
+        s_tok[e] = tok[q];
+        s_scale[e] = f[q];
+      }
+    }
+  }
+  const bool goes_on = tile0 + here < valid && A.keys[tile0 + here] == A.keys[tile0 + here - 1];
+  const bool from_before_tile = tile0 && A.keys[tile0 - 1] == A.keys[tile0];
+  __syncthreads();
+
+  const uint32_t a = min(here, g * S.per_group), b = min(here, a + S.per_group);  // places in the tile
   uint32_t col[NCH];
   bool on[NCH];
 #pragma unroll
@@ -218,119 +269,144 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
       for (int k = 0; k < NCH; ++k)
         if (on[k]) put_sum(A.dtable + (uint64_t)key * S.ds + col[k], acc[k], A.alpha, A.accumulate);
   };
+  // The ring: a lane copies and reads its own chunks only, so it waits for its
+  // own copies and for nobody else.
+  auto ring = [&](uint32_t slot, int u, int k) {
+    return reinterpret_cast<T*>(smem) + (((slot * U + u) * NCH + k) * 256 + threadIdx.x) * V;
+  };
+  auto fetch1 = [&](uint32_t t, uint32_t slot, int u) {
+    const T* row = A.grad + t * S.gs;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+      if (on[k]) {
+        if constexpr (sizeof(T) * V >= 4)
+          cp_async<(int)sizeof(T) * V>(ring(slot, u, k), row + col[k]);
+        else
+          *ring(slot, u, k) = row[col[k]];
+      }
+  };
+  auto fetch = [&](uint32_t p0, uint32_t slot) {
+    if (p0 + U <= b) {
+#pragma unroll
+      for (int u = 0; u < U; u += 4) {
+        const uint4 t = *reinterpret_cast<const uint4*>(s_tok + p0 + u);
+        fetch1(t.x, slot, u);
+        fetch1(t.y, slot, u + 1);
+        fetch1(t.z, slot, u + 2);
+        fetch1(t.w, slot, u + 3);
+      }
+    } else {
+#pragma unroll 1
+      for (int u = 0; p0 + u < b; ++u) fetch1(s_tok[p0 + u], slot, u);
+    }
+    cp_async_commit();
+  };
 
-  bool started = a < b && (a == 0 || A.keys[a - 1] != A.keys[a]);
-  uint32_t cur = a < b ? A.keys[a] : S.rows;
+  bool started = a < b && (a ? s_key[a - 1] != s_key[a] : !from_before_tile);
+  uint32_t cur = a < b ? s_key[a] : S.rows;
   uint32_t hkind = 0;
   Raw<T, V> trow[NCH];  // the table's row of `cur`
-  auto load_row = [&](Raw<T, V> (&r)[NCH], const T* base, uint64_t at, bool in) {
+  auto load_row = [&](Raw<T, V> (&r)[NCH], uint32_t key) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       r[k].zero();
-      if (in && on[k]) r[k].load(base + at + col[k]);
+      if (key < S.rows && on[k]) r[k].load(A.table + key * S.ts + col[k]);
     }
   };
-  if constexpr (DSCALE) load_row(trow, A.table, cur * S.ts, cur < S.rows);
+  auto take = [&](Raw<T, V> (&r)[NCH], uint32_t slot, int u) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      r[k].zero();
+      if (on[k]) r[k].read(ring(slot, u, k));
+    }
+  };
+  auto add = [&](const Raw<T, V> (&r)[NCH], float f) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[k][v] = fmaf(f, r[k].get(v), acc[k][v]);
+  };
+  auto times = [&](const Raw<T, V> (&x)[NCH], const Raw<T, V> (&y)[NCH]) {
+    float d = 0.f;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) d = fmaf(x[k].get(v), y[k].get(v), d);
+    return d;
+  };
+  fetch(a, 0);
+  if constexpr (DSCALE) load_row(trow, cur);
 
-  const bool wide = S.wide_plan;
-  const uint32_t steps = S.per_group / U;  // the same for all lanes: exchanges inside
+  const uint32_t steps = (S.per_group + U - 1) / U;  // the same for all lanes: exchanges inside
   for (uint32_t step = 0; step < steps; ++step) {
-    const uint32_t p0 = a + step * U;
+    const uint32_t p0 = a + step * U, slot = step & 1;
     if (__all_sync(0xffffffffu, p0 >= b)) break;
-    uint32_t key[U], tok[U];
-    float f[U];
-    Raw<T, V> row[U][NCH];
-    if (p0 + U <= b) {
-      load4(A.keys + p0, wide, key, 0);
-      load4(A.keys + p0, wide, key, 4);
-      load4(A.order + p0, wide, tok, 0);
-      load4(A.order + p0, wide, tok, 4);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool in = p0 + u < b;
-        key[u] = in ? A.keys[p0 + u] : S.rows;
-        tok[u] = in ? A.order[p0 + u] : S.n;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = tok[u] < S.n;
-      f[u] = in ? (A.scale ? A.scale[tok[u]] : 1.f) : 0.f;
-      load_row(row[u], A.grad, tok[u] * S.gs, in);
-    }
-    // bit u: place p0 + u begins a key
-    uint32_t begins = 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (p0 + u < b && key[u] != (u ? key[u - 1] : cur)) begins |= 1u << u;
+    cp_async_wait<0>();
+    fetch(p0 + U, slot ^ 1);
     float dot[U];
-    if constexpr (DSCALE) {
-      if (begins == 0) {
+    // sorted: all of them are of the current key when the last is
+    if (p0 + U <= b && s_key[p0 + U - 1] == cur) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          dot[u] = 0.f;
+      for (int u = 0; u < U; u += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(s_scale + p0 + u);
 #pragma unroll
-          for (int k = 0; k < NCH; ++k)
-#pragma unroll
-            for (int v = 0; v < V; ++v) dot[u] = fmaf(row[u][k].get(v), trow[k].get(v), dot[u]);
+        for (int q = 0; q < 4; ++q) {
+          Raw<T, V> row[NCH];
+          take(row, slot, u + q);
+          add(row, q == 0 ? f.x : q == 1 ? f.y : q == 2 ? f.z : f.w);
+          if constexpr (DSCALE) dot[u + q] = times(row, trow);
         }
-      } else {
+      }
+    } else {
+      if constexpr (DSCALE) {
         Raw<T, V> other[U][NCH];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_row(other[u], A.table, key[u] * S.ts, key[u] < S.rows);
+        for (int u = 0; u < U; ++u) load_row(other[u], p0 + u < b ? s_key[p0 + u] : S.rows);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           dot[u] = 0.f;
-#pragma unroll
-          for (int k = 0; k < NCH; ++k)
-#pragma unroll
-            for (int v = 0; v < V; ++v) dot[u] = fmaf(row[u][k].get(v), other[u][k].get(v), dot[u]);
+          if (p0 + u < b) {
+            Raw<T, V> row[NCH];
+            take(row, slot, u);
+            dot[u] = times(row, other[u]);
+          }
         }
 #pragma unroll
         for (int k = 0; k < NCH; ++k) trow[k] = other[U - 1][k];  // of the last place's key
       }
-    }
-    // the places up to the next key's first, then that key
-    for (uint32_t from = 0;;) {
-      const uint32_t rest = begins & ~((1u << from) - 1u);
-      const uint32_t to = rest ? __ffs(rest) - 1 : U;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u >= (int)from && u < (int)to) {
-#pragma unroll
-          for (int k = 0; k < NCH; ++k)
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[k][v] = fmaf(f[u], row[u][k].get(v), acc[k][v]);
+#pragma unroll 1
+      for (int u = 0; u < U && p0 + u < b; ++u) {
+        const uint32_t key = s_key[p0 + u];
+        if (key != cur) {
+          if (started) {
+            write(cur);
+          } else {
+            stage(s_head);
+            hkind = 1;
+          }
+          started = true;
+          clear();
+          cur = key;
         }
-      if (!rest) break;
-      if (started) {
-        write(cur);
-      } else {
-        stage(s_head);
-        hkind = 1;
+        Raw<T, V> row[NCH];
+        take(row, slot, u);
+        add(row, s_scale[p0 + u]);
       }
-      started = true;
-      clear();
-      cur = A.keys[p0 + to];
-      begins &= ~(1u << to);
-      from = to;
     }
     if constexpr (DSCALE) {
+      __syncwarp();
       const GroupSums<U> sums(dot, L, l);
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const uint32_t p = p0 + sums.which + k;
-        if (sums.writes && k < sums.values && p < b) {
-          const uint32_t t = A.order[p];
-          if (t < S.n) A.dscale[t] = A.alpha * dot[k];
-        }
+      const uint32_t p = p0 + sums.which;
+      if (sums.writes) {
+#pragma unroll 1
+        for (int k = 0; k < sums.values; ++k)
+          if (p + k < b) A.dscale[s_tok[p + k]] = A.alpha * sums.at(dot, k);
       }
     }
   }
   bool has_tail = false;
   if (a < b) {
-    const bool ends = b == valid || A.keys[b] != cur;
+    const bool ends = b < here ? s_key[b] != cur : !goes_on;
     if (started && ends) {
       write(cur);
     } else if (!started) {
@@ -468,21 +544,23 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
   const uint32_t slabs = (chunks + S.lanes * NCH - 1) / (S.lanes * NCH);
   const uint32_t groups = 256 / S.lanes;
   // Long groups leave fewer sums to join, short ones more blocks: the longest
-  // of 8 to 64 places that still gives every SM eight blocks.
-  S.per_group = 64;
+  // of 8 to 64 places that still gives every SM eight blocks, as long as the
+  // tile's plan fits.
+  S.per_group = std::min(64u, kMaxTile / groups);
   while (S.per_group > 8 &&
          (uint64_t)slabs * ((S.n + (uint64_t)groups * S.per_group - 1) / ((uint64_t)groups * S.per_group)) <
              8ull * c->sm_count)
     S.per_group >>= 1;
   const uint32_t tile = groups * S.per_group;
   S.tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
-  S.wide_plan = aligned(A.keys, 16) && aligned(A.order, 16);
   S.fill_lanes = std::min(32u, pow2_ceil(chunks));
   const uint32_t fill = A.accumulate ? 0 : (uint32_t)(((S.rows + 255ull) / 256 + slabs - 1) / slabs);
   if (S.tiles + fill == 0) return MVR_OK;
   const bool with_dscale = A.dscale && slabs == 1;
   const auto kernel = with_dscale ? lookup_grad_tile_kernel<T, O, V, true> : lookup_grad_tile_kernel<T, O, V, false>;
-  MVR_CUDA(c, launch_pdl(kernel, dim3(S.tiles + fill, slabs), 256, 0, st, A));
+  const size_t smem = grad_smem<T, V>(tile);
+  MVR_CUDA(c, raise_smem_limit((const void*)kernel, smem));
+  MVR_CUDA(c, launch_pdl(kernel, dim3(S.tiles + fill, slabs), 256, smem, st, A));
   if (S.tiles > 1)  // 32 columns a block while the grid stays small: most blocks have nothing to join
     MVR_CUDA(c, launch_pdl(lookup_grad_join_kernel<O>,
                            dim3(S.tiles - 1, std::max(1u, std::min((S.dim + 31) / 32, 32768u / S.tiles))), 256, 0, st, S, tile, A.offsets, A.keys, A.part,
@@ -522,16 +600,10 @@ int mvr_lookup_device(mvr_ctx* h, const void* d_table, int dtype, uint64_t rows,
     return mvr::tok::by_vec<T>(w, [&](auto vec) {
       constexpr int V = decltype(vec)::value;
       const mvr::tok::Flat F = mvr::tok::flat_of(n, dim / V);
-      if (mvr::tok::many(c, F))
-        mvr::tok::lookup_kernel<T, V, 4><<<mvr::tok::blocks_of(F.total, 1024), 256, 0, c->stream>>>(
-            F, (const T*)d_table, (uint32_t)rows, table_stride, d_ids, id_bytes, d_scale, alpha, (T*)d_out,
-            out_stride);
-      else
-        mvr::tok::lookup_kernel<T, V, 1><<<mvr::tok::blocks_of(F.total, 256), 256, 0, c->stream>>>(
-            F, (const T*)d_table, (uint32_t)rows, table_stride, d_ids, id_bytes, d_scale, alpha, (T*)d_out,
-            out_stride);
-      MVR_CUDA(c, cudaGetLastError());
-      return (int)MVR_OK;
+      return id_bytes == 8 ? mvr::tok::lookup_run<T, uint64_t, V>(c, F, d_table, rows, table_stride, d_ids, d_scale,
+                                                                  alpha, d_out, out_stride)
+                           : mvr::tok::lookup_run<T, uint32_t, V>(c, F, d_table, rows, table_stride, d_ids, d_scale,
+                                                                  alpha, d_out, out_stride);
     });
   });
 }
@@ -578,7 +650,7 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
       return mvr::tok::by_vec<T>(w, [&](auto vec) {
         constexpr int V = decltype(vec)::value;
         mvr::tok::GradArgs<T, O, V> A;
-        A.s = {n, v, dim, 0, 0, 0, 0, false, grad_stride, table_stride, dtable_stride};
+        A.s = {n, v, dim, 0, 0, 0, 0, grad_stride, table_stride, dtable_stride};
         A.grad = (const T*)d_grad;
         A.offsets = d_offsets;
         A.order = d_order;

@@ -66,6 +66,25 @@ struct Raw {
     }
   }
 
+  // the same from shared memory
+  __device__ __forceinline__ void read(const T* p) {
+    if constexpr (kBytes == 16) {
+      const uint4 r = *reinterpret_cast<const uint4*>(p);
+      w[0] = r.x;
+      w[1] = r.y;
+      w[2] = r.z;
+      w[3] = r.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 r = *reinterpret_cast<const uint2*>(p);
+      w[0] = r.x;
+      w[1] = r.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const unsigned short*>(p);
+    }
+  }
+
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (kBytes >= 16) {
 #pragma unroll
@@ -121,10 +140,10 @@ struct Raw {
 
 // The row an id names, or `rows` where it names none (negative ids are large
 // as unsigned values).
-__device__ __forceinline__ uint32_t row_of(const void* ids, int id_bytes, uint64_t i, uint32_t rows) {
-  const uint64_t v = id_bytes == 8 ? static_cast<const uint64_t*>(ids)[i]
-                                   : (uint64_t) static_cast<const uint32_t*>(ids)[i];
-  return v < rows ? (uint32_t)v : rows;
+template <class I>
+__device__ __forceinline__ uint32_t row_of(const I* ids, uint64_t i, uint32_t rows) {
+  const I id = ids[i];
+  return id < rows ? (uint32_t)id : rows;
 }
 
 // Sum of x over the lanes of a group (L a power of two up to 256), in lane 0.

@@ -37,8 +37,7 @@ __device__ __forceinline__ uint32_t key_at(const void* src, uint64_t e, uint32_t
   if constexpr (std::is_same_v<I, void>) {
     return __ldcg(static_cast<const uint32_t*>(src) + e);
   } else {
-    const I id = static_cast<const I*>(src)[e];
-    return id < rows ? (uint32_t)id : rows;
+    return row_of(static_cast<const I*>(src), e, rows);
   }
 }
 
