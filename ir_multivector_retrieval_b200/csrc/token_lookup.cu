@@ -9,55 +9,56 @@ namespace {
 // ---- lookup ----------------------------------------------------------------
 //
 // Bound by memory: the table's rows that are named are read, every output row
-// is written. One thread per V elements, numbered through the whole output,
-// so that a warp writes one run of memory whatever the row length; four of
-// them a thread, the block's stride apart, when there is work for all SMs.
-
+// is written. One thread per V elements, numbered through the whole output, so
+// that a warp writes one run of memory whatever the row length; several of
+// them a thread, the block's stride apart, when there is work for all SMs. All
+// ids and scales are asked for before the first is used: the chain from an id
+// to its row is what a block's time consists of.
 template <class T, class I, int V, int UR, bool SCALE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
 lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, const I* __restrict__ ids,
               const float* __restrict__ scale, float alpha, T* __restrict__ out, uint64_t os) {
   const FlatBlock<UR> B(F);
-  uint64_t i[UR];
-  uint32_t c[UR], r[UR];
+  ids += B.row0;
+  if (SCALE) scale += B.row0;
+  out += B.row0 * os;
+  uint32_t i[UR], c[UR], r[UR];
   float f[UR];
-  bool in[UR];
   Raw<T, V> x[UR];
-  // each loop is one wait for memory
 #pragma unroll
-  for (int j = 0; j < UR; ++j) {
-    in[j] = B.at(j, &i[j], &c[j]);
-    if (!in[j]) i[j] = c[j] = 0;  // read, not written
-  }
+  for (int j = 0; j < UR; ++j) B.place(j, &i[j], &c[j]);  // (0, 0) behind the end: read, not written
 #pragma unroll
   for (int j = 0; j < UR; ++j) r[j] = row_of<I>(ids, i[j], rows);
 #pragma unroll
-  for (int j = 0; j < UR; ++j) f[j] = SCALE ? alpha * scale[i[j]] : alpha;
+  for (int j = 0; j < UR; ++j) f[j] = SCALE ? scale[i[j]] : 1.f;
 #pragma unroll
   for (int j = 0; j < UR; ++j) {
     x[j].zero();
-    if (r[j] < rows) x[j].load(table + r[j] * ts + (uint64_t)c[j] * V);
+    if (r[j] < rows) x[j].load(table + r[j] * ts + c[j] * V);
   }
 #pragma unroll
   for (int j = 0; j < UR; ++j) {
-    if (!in[j]) continue;
+    if (!B.in(j)) continue;
     if (r[j] < rows) {
+      const float g = SCALE ? alpha * f[j] : alpha;
       float y[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) y[v] = f[j] * x[j].get(v);
+      for (int v = 0; v < V; ++v) y[v] = g * x[j].get(v);
       x[j].set(y);
     }
-    x[j].store(out + i[j] * os + (uint64_t)c[j] * V);
+    x[j].store(out + i[j] * os + c[j] * V);
   }
 }
 
 template <class T, class I, int V>
-int lookup_run(Ctx* c, const Flat& F, const void* table, uint64_t rows, uint64_t ts, const void* ids,
+int lookup_run(Ctx* c, uint64_t n, uint32_t chunks, const void* table, uint64_t rows, uint64_t ts, const void* ids,
                const float* scale, float alpha, void* out, uint64_t os) {
-  const bool four = many(c, F);
-  const auto kernel = scale ? (four ? lookup_kernel<T, I, V, 4, true> : lookup_kernel<T, I, V, 1, true>)
-                            : (four ? lookup_kernel<T, I, V, 4, false> : lookup_kernel<T, I, V, 1, false>);
-  kernel<<<blocks_of(F.total, four ? 1024 : 256), 256, 0, c->stream>>>(
+  constexpr int kMany = 4;
+  const Flat F = flat_of(n, chunks);
+  const bool several = F.total >= (uint64_t)kMany * 2048 * c->sm_count;
+  const auto kernel = scale ? (several ? lookup_kernel<T, I, V, kMany, true> : lookup_kernel<T, I, V, 1, true>)
+                            : (several ? lookup_kernel<T, I, V, kMany, false> : lookup_kernel<T, I, V, 1, false>);
+  kernel<<<blocks_of(F.total, several ? 256 * kMany : 256), 256, 0, c->stream>>>(
       F, (const T*)table, (uint32_t)rows, ts, (const I*)ids, scale, alpha, (T*)out, os);
   MVR_CUDA(c, cudaGetLastError());
   return MVR_OK;
@@ -86,7 +87,8 @@ struct GradShape {
   uint32_t n, rows, dim;
   uint32_t lanes;     // L: lanes of a group, a power of two
   uint32_t per_group;  // Tg: places of a group
-  uint32_t tiles;      // blocks with places; those behind them fill rows without a token
+  uint32_t fills;      // blocks that fill rows without a token, before those with places
+  uint32_t tiles;
   uint32_t fill_lanes;  // lanes of a row there, a power of two
   uint64_t gs, ts, ds;  // row strides of grad, table, dtable
 };
@@ -115,19 +117,22 @@ __device__ __forceinline__ void put_sum(O* p, const float (&sum)[V], float alpha
   r.store(p);
 }
 
-// Zeros for the rows without a token: a warp looks at 32 rows at once.
+// Zeros for the rows without a token, 64 rows a block, 8 a warp: enough blocks
+// for all SMs to write at once.
+constexpr uint32_t kFillRows = 64;
 template <class O, int V>
 __device__ __forceinline__ void fill_empty_rows(const GradShape& S, const uint32_t* __restrict__ offsets,
                                                 O* __restrict__ dtable) {
-  const uint64_t block = (uint64_t)(blockIdx.x - S.tiles) * gridDim.y + blockIdx.y;
+  const uint64_t block = (uint64_t)blockIdx.x * gridDim.y + blockIdx.y;
   const uint32_t lane = threadIdx.x & 31;
-  const uint64_t v0 = block * 256 + (threadIdx.x & ~31u);
+  const uint64_t v0 = block * kFillRows + (threadIdx.x >> 5) * (kFillRows / 8);
   const uint64_t v = v0 + lane;
-  const uint32_t empty = __ballot_sync(0xffffffffu, v < S.rows && offsets[v] == offsets[v + 1]);
+  const uint32_t empty =
+      __ballot_sync(0xffffffffu, lane < kFillRows / 8 && v < S.rows && offsets[v] == offsets[v + 1]);
   const uint32_t chunks = S.dim / V, L = S.fill_lanes;
   Raw<O, V> z;
   z.zero();
-  for (uint32_t j = lane / L; j < 32; j += 32 / L)
+  for (uint32_t j = lane / L; j < kFillRows / 8; j += 32 / L)
     if (empty >> j & 1)
       for (uint32_t c = lane & (L - 1); c < chunks; c += L) z.store(dtable + (v0 + j) * S.ds + (uint64_t)c * V);
 }
@@ -193,15 +198,16 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   __shared__ uint32_t s_tkey[256];
   grid_dependency_wait();
   const GradShape& S = A.s;
-  if (blockIdx.x >= S.tiles) {
+  if (blockIdx.x < S.fills) {
     fill_empty_rows<O, V>(S, A.offsets, A.dtable);
     return;
   }
+  const uint32_t tile_at = blockIdx.x - S.fills;
   const uint32_t L = S.lanes, G = 256 / L;
   const uint32_t g = threadIdx.x / L, l = threadIdx.x & (L - 1);
   const uint32_t valid = min(A.offsets[S.rows], S.n);
   const uint32_t tile = G * S.per_group;
-  const uint64_t tile0 = (uint64_t)blockIdx.x * tile;
+  const uint64_t tile0 = (uint64_t)tile_at * tile;
   if constexpr (DSCALE) {  // the tokens behind the last place name no row
     const uint64_t end = min((uint64_t)S.n, tile0 + tile);
     for (uint64_t p = max((uint64_t)valid, tile0) + threadIdx.x; p < end; p += 256)
@@ -225,8 +231,11 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       if (tok[q] >= S.n) tok[q] = 0;  // in bounds whatever the plan holds
-      f[q] = A.scale ? A.scale[tok[q]] : 1.f;
+      f[q] = 1.f;
     }
+    if (A.scale)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[q] = A.scale[tok[q]];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const uint32_t e = e0 + q * 256 + threadIdx.x;
@@ -446,7 +455,7 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
     if (turn == 1 && !open) {
       write(s_tkey[g]);
     } else {
-      float* out = A.part + ((uint64_t)blockIdx.x * 2 + (open ? 1 : 0)) * S.dim;
+      float* out = A.part + ((uint64_t)tile_at * 2 + (open ? 1 : 0)) * S.dim;
 #pragma unroll
       for (int k = 0; k < NCH; ++k)
         if (on[k])
@@ -458,8 +467,8 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
 
 // Block t sums the key that crosses the border of tiles t and t + 1 and has
 // crossed no earlier one: what it left behind the tiles, in their order (the
-// warps take every eighth), then its end.
-template <class O>
+// warps take every eighth), then its end. W columns a lane.
+template <class O, int W>
 __global__ void __launch_bounds__(256)
 lookup_grad_join_kernel(GradShape S, uint32_t tile, const uint32_t* __restrict__ offsets,
                         const uint32_t* __restrict__ keys, const float* __restrict__ part, O* __restrict__ dtable,
@@ -470,23 +479,35 @@ lookup_grad_join_kernel(GradShape S, uint32_t tile, const uint32_t* __restrict__
   if (key >= S.rows || before != key) return;
   const uint32_t first = offsets[key] / tile, last = min((offsets[key + 1] - 1) / tile, S.tiles - 1);
   if (first != blockIdx.x) return;
-  __shared__ float s_sum[256];
+  __shared__ float s_sum[8][W][32];
   const uint32_t w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  for (uint32_t c0 = blockIdx.y * 32; c0 < S.dim; c0 += gridDim.y * 32) {
-    const uint32_t c = c0 + l;
-    float acc = 0.f;
+  for (uint32_t c0 = blockIdx.y * (32 * W); c0 < S.dim; c0 += gridDim.y * (32 * W)) {
+    const uint32_t c = c0 + l * W;
+    float acc[W];
+    Raw<float, W> x;
+#pragma unroll
+    for (int v = 0; v < W; ++v) acc[v] = 0.f;
     if (c < S.dim) {
-#pragma unroll 8
-      for (uint32_t t = first + w; t < last; t += 8) acc += part[((uint64_t)t * 2 + 1) * S.dim + c];
+#pragma unroll 4
+      for (uint32_t t = first + w; t < last; t += 8) {
+        x.load(part + ((uint64_t)t * 2 + 1) * S.dim + c);
+#pragma unroll
+        for (int v = 0; v < W; ++v) acc[v] += x.get(v);
+      }
     }
-    s_sum[threadIdx.x] = acc;
+#pragma unroll
+    for (int v = 0; v < W; ++v) s_sum[w][v][l] = acc[v];
     __syncthreads();
     if (w == 0 && c < S.dim) {
+      x.load(part + (uint64_t)last * 2 * S.dim + c);
 #pragma unroll
-      for (int q = 1; q < 8; ++q) acc += s_sum[q * 32 + l];
-      acc += part[(uint64_t)last * 2 * S.dim + c];
-      const float sum[1] = {acc};
-      put_sum<O, 1>(dtable + (uint64_t)key * S.ds + c, sum, alpha, accumulate);
+      for (int v = 0; v < W; ++v) {
+#pragma unroll
+        for (int q = 1; q < 8; ++q) acc[v] += s_sum[q][v][l];
+        acc[v] += x.get(v);
+        const float sum[1] = {acc[v]};
+        put_sum<O, 1>(dtable + (uint64_t)key * S.ds + c + v, sum, alpha, accumulate);
+      }
     }
     __syncthreads();
   }
@@ -554,17 +575,20 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
   const uint32_t tile = groups * S.per_group;
   S.tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
   S.fill_lanes = std::min(32u, pow2_ceil(chunks));
-  const uint32_t fill = A.accumulate ? 0 : (uint32_t)(((S.rows + 255ull) / 256 + slabs - 1) / slabs);
-  if (S.tiles + fill == 0) return MVR_OK;
+  S.fills = A.accumulate ? 0 : (uint32_t)(((S.rows + kFillRows - 1ull) / kFillRows + slabs - 1) / slabs);
+  if (S.tiles + S.fills == 0) return MVR_OK;
   const bool with_dscale = A.dscale && slabs == 1;
   const auto kernel = with_dscale ? lookup_grad_tile_kernel<T, O, V, true> : lookup_grad_tile_kernel<T, O, V, false>;
   const size_t smem = grad_smem<T, V>(tile);
   MVR_CUDA(c, raise_smem_limit((const void*)kernel, smem));
-  MVR_CUDA(c, launch_pdl(kernel, dim3(S.tiles + fill, slabs), 256, smem, st, A));
-  if (S.tiles > 1)  // 32 columns a block while the grid stays small: most blocks have nothing to join
-    MVR_CUDA(c, launch_pdl(lookup_grad_join_kernel<O>,
-                           dim3(S.tiles - 1, std::max(1u, std::min((S.dim + 31) / 32, 32768u / S.tiles))), 256, 0, st, S, tile, A.offsets, A.keys, A.part,
-                           A.dtable, A.alpha, A.accumulate));
+  MVR_CUDA(c, launch_pdl(kernel, dim3(S.fills + S.tiles, slabs), 256, smem, st, A));
+  if (S.tiles > 1) {  // a block's columns once, while the grid stays small: most blocks have nothing to join
+    const uint32_t w = S.dim % 4 == 0 ? 4 : 1, columns = (S.dim + 32 * w - 1) / (32 * w);
+    const dim3 grid(S.tiles - 1, std::max(1u, std::min(columns, 32768u / S.tiles)));
+    const auto join = w == 4 ? lookup_grad_join_kernel<O, 4> : lookup_grad_join_kernel<O, 1>;
+    MVR_CUDA(c, launch_pdl(join, grid, 256, 0, st, S, tile, A.offsets, A.keys, A.part, A.dtable, A.alpha,
+                           A.accumulate));
+  }
   if (A.dscale && S.tiles && !with_dscale) {  // a row's parts lie in several blocks
     const uint32_t L = lanes_of(c, S.n, chunks);
     lookup_dscale_kernel<T, V><<<blocks_of(S.n, 256 / L), 256, 0, st>>>(L, chunks, A.grad, S.gs, S.n, S.rows, A.keys,
@@ -599,11 +623,8 @@ int mvr_lookup_device(mvr_ctx* h, const void* d_table, int dtype, uint64_t rows,
     using T = std::remove_pointer_t<decltype(t)>;
     return mvr::tok::by_vec<T>(w, [&](auto vec) {
       constexpr int V = decltype(vec)::value;
-      const mvr::tok::Flat F = mvr::tok::flat_of(n, dim / V);
-      return id_bytes == 8 ? mvr::tok::lookup_run<T, uint64_t, V>(c, F, d_table, rows, table_stride, d_ids, d_scale,
-                                                                  alpha, d_out, out_stride)
-                           : mvr::tok::lookup_run<T, uint32_t, V>(c, F, d_table, rows, table_stride, d_ids, d_scale,
-                                                                  alpha, d_out, out_stride);
+      const auto run = id_bytes == 8 ? mvr::tok::lookup_run<T, uint64_t, V> : mvr::tok::lookup_run<T, uint32_t, V>;
+      return run(c, n, dim / V, d_table, rows, table_stride, d_ids, d_scale, alpha, d_out, out_stride);
     });
   });
 }
@@ -650,7 +671,7 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
       return mvr::tok::by_vec<T>(w, [&](auto vec) {
         constexpr int V = decltype(vec)::value;
         mvr::tok::GradArgs<T, O, V> A;
-        A.s = {n, v, dim, 0, 0, 0, 0, grad_stride, table_stride, dtable_stride};
+        A.s = {n, v, dim, 0, 0, 0, 0, 0, grad_stride, table_stride, dtable_stride};
         A.grad = (const T*)d_grad;
         A.offsets = d_offsets;
         A.order = d_order;

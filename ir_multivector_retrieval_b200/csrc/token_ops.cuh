@@ -179,6 +179,14 @@ struct FlatBlock {
     row0 = F.shift >= 0 ? first >> F.shift : first / F.chunks;
     rem0 = (uint32_t)(first - row0 * F.chunks);
   }
+  __device__ __forceinline__ bool in(int j) const { return first + (j * 256 + threadIdx.x) < F.total; }
+  // the row from row0 on, and the chunk; (0, 0) behind the end
+  __device__ __forceinline__ void place(int j, uint32_t* row, uint32_t* chunk) const {
+    const uint32_t x = rem0 + j * 256 + threadIdx.x;
+    const uint32_t q = F.shift >= 0 ? x >> F.shift : x / F.chunks;
+    *row = in(j) ? q : 0;
+    *chunk = in(j) ? x - q * F.chunks : 0;
+  }
   // false behind the end
   __device__ __forceinline__ bool at(int j, uint64_t* row, uint32_t* chunk) const {
     const uint32_t local = j * 256 + threadIdx.x;

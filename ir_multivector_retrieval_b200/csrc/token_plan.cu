@@ -20,7 +20,7 @@ namespace {
 
 constexpr uint32_t kSmallThreads = 1024, kSmallRounds = 8, kSmallBlocks = 8;
 constexpr uint32_t kSmallMax = kSmallThreads * kSmallRounds * kSmallBlocks;  // 65,536 pairs
-constexpr int kSmallBits = 11;                                               // of a digit
+constexpr int kSmallBits = 10;                                               // of a digit
 constexpr uint32_t kTileThreads = 512, kTileRounds = 8, kTile = kTileThreads * kTileRounds;
 constexpr int kTileBits = 10;
 
@@ -41,26 +41,33 @@ __device__ __forceinline__ uint32_t key_at(const void* src, uint64_t e, uint32_t
   }
 }
 
-// Equal digits among the warp's lanes that are `in`: how many are below this
-// lane, and how many there are. (One vote a bit of the digit measured slower.)
-struct Peers {
-  uint32_t below, count;
-  __device__ __forceinline__ Peers(uint32_t digit, bool in) {
-    const uint32_t m = __match_any_sync(0xffffffffu, in ? digit : ~(threadIdx.x & 31));
-    below = __popc(m & lanemask_lt());
-    count = __popc(m);
-  }
-};
+// Places of a warp's pairs among its pairs of the same digit, round by round:
+// the first lane of those that share a digit adds their number to the count.
+// (Voting on each bit of the digit instead of matching measured slower.)
+__device__ __forceinline__ uint32_t place_in(uint32_t* count, uint32_t digit, bool in) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t m = __match_any_sync(0xffffffffu, in ? digit : ~lane);
+  const uint32_t first = __ffs(m) - 1;
+  uint32_t before = 0;
+  if (in && lane == first) before = atomicAdd(count + digit, __popc(m));
+  __syncwarp();  // the next round's additions come after this one's
+  return __shfl_sync(0xffffffffu, before, first) + __popc(m & lanemask_lt());
+}
 
 // A digit's counts in the warps' rows of s, R apart, become those of the warps
 // before; their sum.
-__device__ __forceinline__ uint32_t warps_prefix(uint16_t* s, uint32_t R, uint32_t warps) {
+__device__ __forceinline__ uint32_t warps_prefix(uint32_t* s, uint32_t R, uint32_t warps) {
   uint32_t run = 0;
-#pragma unroll 4
-  for (uint32_t q = 0; q < warps; ++q) {
-    const uint32_t x = s[q * R];
-    s[q * R] = (uint16_t)run;
-    run += x;
+#pragma unroll 1
+  for (uint32_t q = 0; q < warps; q += 4) {  // warps come in fours
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = s[(q + k) * R];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s[(q + k) * R] = run;
+      run += x[k];
+    }
   }
   return run;
 }
@@ -121,8 +128,8 @@ plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint3
   uint32_t* s_total = smem;       // [R] the block's pairs of a digit
   uint32_t* s_base = s_total + R;  // [R] first place of the digit
   uint32_t* s_before = s_base + R;  // [R] its pairs in the blocks before
-  uint16_t* s_count = reinterpret_cast<uint16_t*>(s_before + R);  // [warps][R] a warp's; then those of the warps before
-  uint16_t* mine = s_count + warp * R;
+  uint32_t* s_count = s_before + R;  // [warps][R] a warp's; then those of the warps before
+  uint32_t* mine = s_count + warp * R;
   const uint32_t first = rank * (rounds * threads) + warp * (rounds * 32) + lane;
   const uint32_t *kin = nullptr, *vin = nullptr;
   uint32_t *kout = k0, *vout = v0;
@@ -140,24 +147,19 @@ plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint3
         val[j] = pass ? __ldcg(vin + e) : e;
       }
     }
-    for (uint32_t e = t; e < warps * R / 2; e += threads) reinterpret_cast<uint32_t*>(s_count)[e] = 0;
+    for (uint32_t e = t; e < warps * R; e += threads) s_count[e] = 0;
     __syncthreads();
 #pragma unroll
     for (uint32_t j = 0; j < kSmallRounds; ++j) {
       if (j >= rounds) break;
-      const bool in = first + j * 32 < A.n;
-      const uint32_t d = (key[j] >> shift) & (R - 1);
-      const Peers p(d, in);
-      if (in) place[j] = mine[d] + p.below;
-      __syncwarp();
-      if (in && p.below == 0) mine[d] += (uint16_t)p.count;
-      __syncwarp();
+      place[j] = place_in(mine, (key[j] >> shift) & (R - 1), first + j * 32 < A.n);
     }
     __syncthreads();
     for (uint32_t d = t; d < R; d += threads) s_total[d] = warps_prefix(s_count + d, R, warps);
     cluster.sync();
     for (uint32_t d = t; d < R; d += threads) {
       uint32_t before = 0, all = 0;
+#pragma unroll 2
       for (uint32_t q = 0; q < blocks; ++q) {
         const uint32_t x = *cluster.map_shared_rank(s_total + d, q);
         if (q < rank) before += x;
@@ -244,52 +246,41 @@ plan_scan_kernel(uint32_t tiles, uint32_t* __restrict__ hist, uint32_t* __restri
 }
 
 // A tile's pairs, sorted by digit in shared memory first so that each digit's
-// run is written in one piece.
+// run is written in one piece. 42 registers a thread let three blocks share an
+// SM, so that up to 1.8 million pairs are one wave of blocks.
 template <class I, bool LAST>
-__global__ void __launch_bounds__(kTileThreads)
+__global__ void __launch_bounds__(kTileThreads, 3)
 plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __restrict__ vin, int shift,
                     int bits, uint32_t tiles, const uint32_t* __restrict__ hist,
                     const uint32_t* __restrict__ total, uint32_t* __restrict__ kout, uint32_t* __restrict__ vout) {
   constexpr uint32_t kWarps = kTileThreads / 32;
   const uint32_t R = 1u << bits;
   extern __shared__ uint32_t smem[];
-  uint32_t* s_key = smem;              // [kTile]
-  uint32_t* s_val = s_key + kTile;     // [kTile]
-  uint32_t* s_start = s_val + kTile;   // [R] first place of the digit in the tile
+  uint32_t* s_start = smem;            // [R] first place of the digit in the tile
   uint32_t* s_glob = s_start + R;      // [R] its first place among all, less s_start
-  uint16_t* s_count = reinterpret_cast<uint16_t*>(s_glob + R);  // [kWarps][R]
+  uint32_t* s_count = s_glob + R;      // [kWarps][R] a warp's; then those of the warps before
+  uint32_t* s_key = s_count;           // [kTile] once the places are known
+  uint32_t* s_val = s_key + kTile;     // [kTile]
   __shared__ uint32_t s_warp[32];
   grid_dependency_wait();
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  for (uint32_t e = t; e < kWarps * R; e += kTileThreads) s_count[e] = 0;
-  for (uint32_t d = t; d < R; d += kTileThreads) s_glob[d] = total[d];
   const uint64_t tile0 = (uint64_t)blockIdx.x * kTile;
   const uint32_t in_tile = (uint32_t)min((uint64_t)kTile, A.n - tile0);
   const uint32_t first = warp * (kTileRounds * 32) + lane;
-  uint32_t key[kTileRounds], val[kTileRounds], place[kTileRounds];
+  uint32_t key[kTileRounds], place[kTileRounds];
 #pragma unroll
   for (uint32_t j = 0; j < kTileRounds; ++j) {
     const uint32_t q = first + j * 32;
-    key[j] = val[j] = 0;
-    if (q < in_tile) {
-      key[j] = key_at<I>(src, tile0 + q, A.rows);
-      val[j] = std::is_same_v<I, void> ? __ldcg(vin + tile0 + q) : (uint32_t)(tile0 + q);
-    }
+    key[j] = q < in_tile ? key_at<I>(src, tile0 + q, A.rows) : 0;
   }
+  for (uint32_t e = t; e < kWarps * R; e += kTileThreads) s_count[e] = 0;
+  for (uint32_t d = t; d < R; d += kTileThreads) s_glob[d] = total[d];
   __syncthreads();
-  block_prefix(s_glob, R, kTileThreads, s_warp);
-  uint16_t* mine = s_count + warp * R;
+  uint32_t* mine = s_count + warp * R;
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j) {
-    const bool in = first + j * 32 < in_tile;
-    const uint32_t d = (key[j] >> shift) & (R - 1);
-    const Peers p(d, in);
-    if (in) place[j] = mine[d] + p.below;
-    __syncwarp();
-    if (in && p.below == 0) mine[d] += (uint16_t)p.count;
-    __syncwarp();
-  }
-  __syncthreads();
+  for (uint32_t j = 0; j < kTileRounds; ++j)
+    place[j] = place_in(mine, (key[j] >> shift) & (R - 1), first + j * 32 < in_tile);
+  block_prefix(s_glob, R, kTileThreads, s_warp);
   for (uint32_t d = t; d < R; d += kTileThreads) s_start[d] = warps_prefix(s_count + d, R, kWarps);
   __syncthreads();
   block_prefix(s_start, R, kTileThreads, s_warp);
@@ -297,11 +288,16 @@ plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __
     s_glob[d] += hist[(uint64_t)d * tiles + blockIdx.x] - s_start[d];
 #pragma unroll
   for (uint32_t j = 0; j < kTileRounds; ++j) {
-    if (first + j * 32 < in_tile) {
-      const uint32_t d = (key[j] >> shift) & (R - 1);
-      const uint32_t q = s_start[d] + mine[d] + place[j];
-      s_key[q] = key[j];
-      s_val[q] = val[j];
+    const uint32_t d = (key[j] >> shift) & (R - 1);
+    place[j] += s_start[d] + mine[d];
+  }
+  __syncthreads();  // the counts' memory holds the pairs from here on
+#pragma unroll
+  for (uint32_t j = 0; j < kTileRounds; ++j) {
+    const uint32_t q = first + j * 32;
+    if (q < in_tile) {
+      s_key[place[j]] = key[j];
+      s_val[place[j]] = std::is_same_v<I, void> ? __ldcg(vin + tile0 + q) : (uint32_t)(tile0 + q);
     }
   }
   __syncthreads();
@@ -343,39 +339,52 @@ __global__ void __launch_bounds__(256) plan_offsets_kernel(PlanArgs A) {
 // behind the key before it up to its own. Gaps up to kOwnFill are filled by
 // their thread, up to kWarpFill by its warp, longer ones by the block.
 constexpr uint32_t kOwnFill = 4, kWarpFill = 1024;
+constexpr uint32_t kBorderPlaces = 1024;  // of a block
 __global__ void __launch_bounds__(256) plan_borders_kernel(PlanArgs A) {
-  __shared__ uint32_t s_gaps, s_lo[256], s_hi[256], s_place[256];
+  __shared__ uint32_t s_gaps, s_lo[kBorderPlaces], s_hi[kBorderPlaces], s_place[kBorderPlaces];
   grid_dependency_wait();
   if (threadIdx.x == 0) s_gaps = 0;
   __syncthreads();
   const uint32_t lane = threadIdx.x & 31;
-  const uint64_t p = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  uint32_t lo = 0, hi = 0;  // rows to fill
-  if (p <= A.n) {
-    lo = p ? A.keys[p - 1] + 1 : 0;
-    hi = p < A.n ? A.keys[p] + 1 : A.rows + 1;
+  constexpr int Q = kBorderPlaces / 256;
+  const uint64_t p0 = (uint64_t)blockIdx.x * kBorderPlaces + threadIdx.x;
+  uint32_t lo[Q], hi[Q];  // rows to fill
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    const uint64_t p = p0 + q * 256;
+    lo[q] = hi[q] = 0;
+    if (p <= A.n) {
+      if (p) lo[q] = A.keys[p - 1] + 1;
+      hi[q] = p < A.n ? A.keys[p] + 1 : A.rows + 1;
+    }
   }
-  const uint32_t gap = lo < hi ? hi - lo : 0;
-  if (gap <= kOwnFill) {
-    for (uint32_t v = lo; v < lo + gap; ++v) A.offsets[v] = (uint32_t)p;
-  } else if (gap > kWarpFill) {
-    const uint32_t g = atomicAdd(&s_gaps, 1u);
-    s_lo[g] = lo;
-    s_hi[g] = hi;
-    s_place[g] = (uint32_t)p;
-  }
-  uint32_t todo = __ballot_sync(0xffffffffu, gap > kOwnFill && gap <= kWarpFill);
-  while (todo) {
-    const int l = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const uint32_t from = __shfl_sync(0xffffffffu, lo, l), to = __shfl_sync(0xffffffffu, hi, l);
-    const uint32_t place = __shfl_sync(0xffffffffu, (uint32_t)p, l);
-    for (uint32_t v = from + lane; v < to; v += 32) A.offsets[v] = place;
+#pragma unroll 1
+  for (int q = 0; q < Q; ++q) {
+    const uint32_t from = q == 0 ? lo[0] : q == 1 ? lo[1] : q == 2 ? lo[2] : lo[3];
+    const uint32_t to = q == 0 ? hi[0] : q == 1 ? hi[1] : q == 2 ? hi[2] : hi[3];
+    const uint32_t p = (uint32_t)(p0 + q * 256), gap = from < to ? to - from : 0;
+    if (gap <= kOwnFill) {
+      for (uint32_t v = from; v < from + gap; ++v) A.offsets[v] = p;
+    } else if (gap > kWarpFill) {
+      const uint32_t g = atomicAdd(&s_gaps, 1u);
+      s_lo[g] = from;
+      s_hi[g] = to;
+      s_place[g] = p;
+    }
+    uint32_t todo = __ballot_sync(0xffffffffu, gap > kOwnFill && gap <= kWarpFill);
+    while (todo) {
+      const int l = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const uint32_t a = __shfl_sync(0xffffffffu, from, l), b = __shfl_sync(0xffffffffu, to, l);
+      const uint32_t place = __shfl_sync(0xffffffffu, p, l);
+      for (uint32_t v = a + lane; v < b; v += 32) A.offsets[v] = place;
+    }
   }
   __syncthreads();
   for (uint32_t g = 0; g < s_gaps; ++g)
     for (uint64_t v = (uint64_t)s_lo[g] + threadIdx.x; v < s_hi[g]; v += 256) A.offsets[v] = s_place[g];
 }
+static_assert(kBorderPlaces == 4 * 256, "the loop over a thread's places");
 
 struct Digits {
   int bits, passes;
@@ -417,9 +426,9 @@ int plan_small(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_
   const uint32_t blocks = std::min(kSmallBlocks, pow2_ceil((A.n + 2047) / 2048));
   const uint32_t chunk = (A.n + blocks - 1) / blocks;
   const uint32_t threads =
-      std::min(kSmallThreads, std::max({(chunk + 31) / 32 * 32, std::min(R, 256u), 64u}));
+      std::min(kSmallThreads, std::max((chunk + 127) / 128 * 128, std::min(R, 256u)));
   const uint32_t rounds = (chunk + threads - 1) / threads;
-  const size_t smem = 3 * R * 4 + (size_t)threads / 32 * R * 2;
+  const size_t smem = (3 + (size_t)threads / 32) * R * 4;
   MVR_CUDA(c, raise_smem_limit((const void*)plan_small_kernel<I>, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = blocks;
@@ -442,7 +451,7 @@ int plan_pass(Ctx* c, const PlanArgs& A, const void* kin, const uint32_t* vin, i
               uint32_t* kout, uint32_t* vout, uint32_t* hist, uint32_t* sums) {
   cudaStream_t st = c->stream;
   const uint32_t tiles = (uint32_t)((A.n + (kTile - 1ull)) / kTile), R = 1u << bits;
-  const size_t smem = (2 * kTile + 2 * R) * 4 + kTileThreads / 32 * R * 2;
+  const size_t smem = (2 * R + std::max(kTileThreads / 32 * R, 2 * kTile)) * 4;
   MVR_CUDA(c, launch_pdl(plan_hist_kernel<I>, tiles, kTileThreads, 0, st, kin, A.n, A.rows, shift, R, tiles, hist));
   MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
   const auto scatter = last ? plan_scatter_kernel<I, true> : plan_scatter_kernel<I, false>;
@@ -515,7 +524,8 @@ int mvr_token_plan_device(mvr_ctx* h, const void* d_ids, int id_bytes, uint64_t 
   // Walking the places costs one read each, a search some twenty dependent ones
   // a row: the walk is for rows that do not outnumber the places by far.
   if (rows <= 8 * n_ids)
-    MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_borders_kernel, (unsigned)(n_ids / 256 + 1), 256, 0, st, A));
+    MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_borders_kernel, (unsigned)(n_ids / mvr::tok::kBorderPlaces + 1),
+                                  256, 0, st, A));
   else
     MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_offsets_kernel, (unsigned)(rows / 256 + 1), 256, 0, st, A));
   return MVR_OK;
