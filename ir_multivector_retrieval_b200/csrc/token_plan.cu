@@ -15,14 +15,14 @@ namespace {
 // The sort is by radix, stable: in each pass, least significant digit first, a
 // pair goes to (pairs of smaller digits) + (pairs of its digit before it). The
 // ids are a few bytes a token beside rows of hundreds, so what costs is the
-// number of dependent steps: up to kSmallMax pairs one cluster of blocks does
-// all passes in one launch; above, a pass is three launches over tiles.
+// number of dependent steps: some thousand pairs go through all passes in
+// one launch of one cluster of blocks; above, a pass is three launches over tiles.
 
-constexpr uint32_t kSmallThreads = 1024, kSmallRounds = 8, kSmallBlocks = 8;
-constexpr uint32_t kSmallMax = kSmallThreads * kSmallRounds * kSmallBlocks;  // 65,536 pairs
-constexpr int kSmallBits = 10;                                               // of a digit
-constexpr uint32_t kTileThreads = 512, kTileRounds = 8, kTile = kTileThreads * kTileRounds;
-constexpr int kTileBits = 10;
+constexpr int kMostBits = 10;  // of a digit
+constexpr uint32_t kSmallThreads = 256, kSmallRounds = 8, kSmallBlocks = 8;
+constexpr uint32_t kSmallMax = kSmallThreads * kSmallRounds * kSmallBlocks;  // 16,384 pairs
+constexpr uint32_t kSmallMaxPasses = kSmallMax / 2;                          // where one pass is not enough
+constexpr uint32_t kTileThreads = 512;
 
 struct PlanArgs {
   const void* ids;
@@ -41,17 +41,26 @@ __device__ __forceinline__ uint32_t key_at(const void* src, uint64_t e, uint32_t
   }
 }
 
-// Places of a warp's pairs among its pairs of the same digit, round by round:
-// the first lane of those that share a digit adds their number to the count.
-// (Voting on each bit of the digit instead of matching measured slower.)
-__device__ __forceinline__ uint32_t place_in(uint32_t* count, uint32_t digit, bool in) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint32_t m = __match_any_sync(0xffffffffu, in ? digit : ~lane);
-  const uint32_t first = __ffs(m) - 1;
-  uint32_t before = 0;
-  if (in && lane == first) before = atomicAdd(count + digit, __popc(m));
-  __syncwarp();  // the next round's additions come after this one's
-  return __shfl_sync(0xffffffffu, before, first) + __popc(m & lanemask_lt());
+// Place of a lane's pair among its warp's pairs of the same digit so far; the
+// warp's count of the digit goes up by this round's. Lanes with equal digits
+// are found by a vote on each bit: 30 cycles of the SM a warp at 8 bits, where
+// the match instruction takes 66 when the digits differ.
+__device__ __forceinline__ uint32_t place_in(uint32_t* count, uint32_t digit, int bits, bool in) {
+  uint32_t m = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+  for (int b = 0; b < kMostBits; ++b)
+    if (b < bits) {
+      const bool one = digit >> b & 1;
+      const uint32_t v = __ballot_sync(0xffffffffu, one);
+      m &= one ? v : ~v;
+    }
+  const uint32_t below = __popc(m & lanemask_lt());
+  uint32_t place = 0;
+  if (in) place = count[digit] + below;
+  __syncwarp();
+  if (in && below == 0) count[digit] += __popc(m);
+  __syncwarp();
+  return place;
 }
 
 // A digit's counts in the warps' rows of s, R apart, become those of the warps
@@ -152,7 +161,7 @@ plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint3
 #pragma unroll
     for (uint32_t j = 0; j < kSmallRounds; ++j) {
       if (j >= rounds) break;
-      place[j] = place_in(mine, (key[j] >> shift) & (R - 1), first + j * 32 < A.n);
+      place[j] = place_in(mine, (key[j] >> shift) & (R - 1), digit_bits, first + j * 32 < A.n);
     }
     __syncthreads();
     for (uint32_t d = t; d < R; d += threads) s_total[d] = warps_prefix(s_count + d, R, warps);
@@ -195,24 +204,24 @@ plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint3
 }
 
 // Pairs of each digit in a tile: hist[digit][tile].
-template <class I>
+template <class I, uint32_t ROUNDS>
 __global__ void __launch_bounds__(kTileThreads)
 plan_hist_kernel(const void* __restrict__ src, uint32_t n, uint32_t rows, int shift, uint32_t R, uint32_t tiles,
                  uint32_t* __restrict__ hist) {
-  __shared__ uint32_t s_count[1 << kTileBits];
+  __shared__ uint32_t s_count[1 << kMostBits];
   grid_dependency_wait();
   const uint32_t t = threadIdx.x;
   for (uint32_t d = t; d < R; d += kTileThreads) s_count[d] = 0;
   __syncthreads();
-  const uint64_t first = (uint64_t)blockIdx.x * kTile + t;
-  uint32_t key[kTileRounds];
+  const uint64_t first = (uint64_t)blockIdx.x * (kTileThreads * ROUNDS) + t;
+  uint32_t key[ROUNDS];
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j) {
+  for (uint32_t j = 0; j < ROUNDS; ++j) {
     const uint64_t e = first + j * kTileThreads;
     key[j] = e < n ? key_at<I>(src, e, rows) : ~0u;
   }
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j)
+  for (uint32_t j = 0; j < ROUNDS; ++j)
     if (first + j * kTileThreads < n) atomicAdd(&s_count[(key[j] >> shift) & (R - 1)], 1u);
   __syncthreads();
   for (uint32_t d = t; d < R; d += kTileThreads) hist[(uint64_t)d * tiles + blockIdx.x] = s_count[d];
@@ -248,12 +257,12 @@ plan_scan_kernel(uint32_t tiles, uint32_t* __restrict__ hist, uint32_t* __restri
 // A tile's pairs, sorted by digit in shared memory first so that each digit's
 // run is written in one piece. 42 registers a thread let three blocks share an
 // SM, so that up to 1.8 million pairs are one wave of blocks.
-template <class I, bool LAST>
+template <class I, uint32_t ROUNDS, bool LAST>
 __global__ void __launch_bounds__(kTileThreads, 3)
 plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __restrict__ vin, int shift,
                     int bits, uint32_t tiles, const uint32_t* __restrict__ hist,
                     const uint32_t* __restrict__ total, uint32_t* __restrict__ kout, uint32_t* __restrict__ vout) {
-  constexpr uint32_t kWarps = kTileThreads / 32;
+  constexpr uint32_t kWarps = kTileThreads / 32, kTile = kTileThreads * ROUNDS;
   const uint32_t R = 1u << bits;
   extern __shared__ uint32_t smem[];
   uint32_t* s_start = smem;            // [R] first place of the digit in the tile
@@ -266,10 +275,10 @@ plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __
   const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint64_t tile0 = (uint64_t)blockIdx.x * kTile;
   const uint32_t in_tile = (uint32_t)min((uint64_t)kTile, A.n - tile0);
-  const uint32_t first = warp * (kTileRounds * 32) + lane;
-  uint32_t key[kTileRounds], place[kTileRounds];
+  const uint32_t first = warp * (ROUNDS * 32) + lane;
+  uint32_t key[ROUNDS], place[ROUNDS];
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j) {
+  for (uint32_t j = 0; j < ROUNDS; ++j) {
     const uint32_t q = first + j * 32;
     key[j] = q < in_tile ? key_at<I>(src, tile0 + q, A.rows) : 0;
   }
@@ -278,8 +287,8 @@ plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __
   __syncthreads();
   uint32_t* mine = s_count + warp * R;
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j)
-    place[j] = place_in(mine, (key[j] >> shift) & (R - 1), first + j * 32 < in_tile);
+  for (uint32_t j = 0; j < ROUNDS; ++j)
+    place[j] = place_in(mine, (key[j] >> shift) & (R - 1), bits, first + j * 32 < in_tile);
   block_prefix(s_glob, R, kTileThreads, s_warp);
   for (uint32_t d = t; d < R; d += kTileThreads) s_start[d] = warps_prefix(s_count + d, R, kWarps);
   __syncthreads();
@@ -287,13 +296,13 @@ plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __
   for (uint32_t d = t; d < R; d += kTileThreads)
     s_glob[d] += hist[(uint64_t)d * tiles + blockIdx.x] - s_start[d];
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j) {
+  for (uint32_t j = 0; j < ROUNDS; ++j) {
     const uint32_t d = (key[j] >> shift) & (R - 1);
     place[j] += s_start[d] + mine[d];
   }
   __syncthreads();  // the counts' memory holds the pairs from here on
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j) {
+  for (uint32_t j = 0; j < ROUNDS; ++j) {
     const uint32_t q = first + j * 32;
     if (q < in_tile) {
       s_key[place[j]] = key[j];
@@ -302,7 +311,7 @@ plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __
   }
   __syncthreads();
 #pragma unroll
-  for (uint32_t j = 0; j < kTileRounds; ++j) {
+  for (uint32_t j = 0; j < ROUNDS; ++j) {
     const uint32_t q = j * kTileThreads + t;
     if (q >= in_tile) break;
     const uint32_t k = s_key[q], v = s_val[q];
@@ -336,18 +345,18 @@ __global__ void __launch_bounds__(256) plan_offsets_kernel(PlanArgs A) {
 }
 
 // The same for rows of the places' number: place p (n included) fills the rows
-// behind the key before it up to its own. Gaps up to kOwnFill are filled by
-// their thread, up to kWarpFill by its warp, longer ones by the block.
-constexpr uint32_t kOwnFill = 4, kWarpFill = 1024;
-constexpr uint32_t kBorderPlaces = 1024;  // of a block
+// behind the key before it up to its own. A warp fills the gaps of its 32
+// places as one run of rows, the block one that is longer than kWarpFill.
+// Q: places of a thread, several when there are enough blocks anyway.
+constexpr uint32_t kWarpFill = 1024;
+template <int Q>
 __global__ void __launch_bounds__(256) plan_borders_kernel(PlanArgs A) {
-  __shared__ uint32_t s_gaps, s_lo[kBorderPlaces], s_hi[kBorderPlaces], s_place[kBorderPlaces];
+  __shared__ uint32_t s_gaps, s_lo[256 * Q], s_hi[256 * Q], s_place[256 * Q];
   grid_dependency_wait();
   if (threadIdx.x == 0) s_gaps = 0;
   __syncthreads();
   const uint32_t lane = threadIdx.x & 31;
-  constexpr int Q = kBorderPlaces / 256;
-  const uint64_t p0 = (uint64_t)blockIdx.x * kBorderPlaces + threadIdx.x;
+  const uint64_t p0 = (uint64_t)blockIdx.x * (256 * Q) + threadIdx.x;
   uint32_t lo[Q], hi[Q];  // rows to fill
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
@@ -358,50 +367,74 @@ __global__ void __launch_bounds__(256) plan_borders_kernel(PlanArgs A) {
       hi[q] = p < A.n ? A.keys[p] + 1 : A.rows + 1;
     }
   }
-#pragma unroll 1
+#pragma unroll
   for (int q = 0; q < Q; ++q) {
-    const uint32_t from = q == 0 ? lo[0] : q == 1 ? lo[1] : q == 2 ? lo[2] : lo[3];
-    const uint32_t to = q == 0 ? hi[0] : q == 1 ? hi[1] : q == 2 ? hi[2] : hi[3];
-    const uint32_t p = (uint32_t)(p0 + q * 256), gap = from < to ? to - from : 0;
-    if (gap <= kOwnFill) {
-      for (uint32_t v = from; v < from + gap; ++v) A.offsets[v] = p;
-    } else if (gap > kWarpFill) {
+    const uint32_t p = (uint32_t)(p0 + q * 256);
+    uint32_t gap = lo[q] < hi[q] ? hi[q] - lo[q] : 0;
+    if (gap > kWarpFill) {
       const uint32_t g = atomicAdd(&s_gaps, 1u);
-      s_lo[g] = from;
-      s_hi[g] = to;
+      s_lo[g] = lo[q];
+      s_hi[g] = hi[q];
       s_place[g] = p;
+      gap = 0;
     }
-    uint32_t todo = __ballot_sync(0xffffffffu, gap > kOwnFill && gap <= kWarpFill);
-    while (todo) {
-      const int l = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const uint32_t a = __shfl_sync(0xffffffffu, from, l), b = __shfl_sync(0xffffffffu, to, l);
+    uint32_t end = gap;  // of the gaps up to this lane's
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= (uint32_t)o) end += x;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, end, 31);
+    for (uint32_t f0 = 0; f0 < total; f0 += 32) {
+      const uint32_t f = f0 + lane;
+      uint32_t l = 0;  // the lane whose gap has the f-th row: the first whose end is behind f
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        if (__shfl_sync(0xffffffffu, end, l + o - 1) <= f) l += o;
+      l = min(l, 31u);
+      const uint32_t row = __shfl_sync(0xffffffffu, lo[q] + gap - end, l) + f;
       const uint32_t place = __shfl_sync(0xffffffffu, p, l);
-      for (uint32_t v = a + lane; v < b; v += 32) A.offsets[v] = place;
+      if (f < total) A.offsets[row] = place;
     }
   }
   __syncthreads();
   for (uint32_t g = 0; g < s_gaps; ++g)
     for (uint64_t v = (uint64_t)s_lo[g] + threadIdx.x; v < s_hi[g]; v += 256) A.offsets[v] = s_place[g];
 }
-static_assert(kBorderPlaces == 4 * 256, "the loop over a thread's places");
+
+int plan_borders(Ctx* c, const PlanArgs& A) {
+  const bool four = A.n >= 1024u * 8 * (uint32_t)c->sm_count;
+  const unsigned per = four ? 1024 : 256;
+  MVR_CUDA(c, launch_pdl(four ? plan_borders_kernel<4> : plan_borders_kernel<1>, A.n / per + 1, 256, 0, c->stream, A));
+  return MVR_OK;
+}
 
 struct Digits {
   int bits, passes;
-  Digits(uint64_t rows, int most) {
+  explicit Digits(uint64_t rows) {
     int b = 1;
     while ((rows >> b) != 0) ++b;  // keys are 0 .. rows
-    passes = (b + most - 1) / most;
+    passes = (b + kMostBits - 1) / kMostBits;
     bits = (b + passes - 1) / passes;
   }
 };
+
+// Whether one cluster does it: a pass takes it as long as the tiles' three
+// launches at some 10,000 pairs.
+bool is_small(uint64_t n, const Digits& D) { return n <= (D.passes == 1 ? kSmallMax : kSmallMaxPasses); }
+
+// Pairs a thread of a tile: few while that gives more blocks than share the
+// SMs at once.
+constexpr uint64_t kFewRounds = 2, kManyRounds = 8;
+bool few_rounds(uint64_t n) { return n <= 444 * kFewRounds * kTileThreads; }
 
 // Workspace: two sets of pairs for the passes, and the counts of the tiles.
 struct PlanSpace {
   uint64_t k0, v0, k1, v1, hist, sums, total;
   PlanSpace(uint64_t n, uint64_t rows) {
-    const bool small = n <= kSmallMax;
-    const Digits D(rows, small ? kSmallBits : kTileBits);
+    const Digits D(rows);
+    const bool small = is_small(n, D);
+    const uint64_t tile = kTileThreads * (few_rounds(n) ? kFewRounds : kManyRounds);
     uint64_t off = 0;
     auto take = [&](uint64_t words) {
       const uint64_t o = off;
@@ -412,7 +445,7 @@ struct PlanSpace {
     v0 = take(D.passes > 1 ? n : 0);
     k1 = take(D.passes > 2 ? n : 0);
     v1 = take(D.passes > 2 ? n : 0);
-    hist = take(small ? 0 : ((n + kTile - 1) / kTile) << D.bits);
+    hist = take(small ? 0 : ((n + tile - 1) / tile) << D.bits);
     sums = take(small ? 0 : 1ull << D.bits);
     total = off;
   }
@@ -420,13 +453,10 @@ struct PlanSpace {
 
 template <class I>
 int plan_small(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_t* v0, uint32_t* k1, uint32_t* v1) {
-  // another block joins for every 2048 pairs; a block has the warps that its
-  // pairs fill, and some more for the prefix sums of many digits
-  const uint32_t R = 1u << D.bits;
-  const uint32_t blocks = std::min(kSmallBlocks, pow2_ceil((A.n + 2047) / 2048));
+  // another block joins for every 256 pairs
+  const uint32_t R = 1u << D.bits, threads = kSmallThreads;
+  const uint32_t blocks = std::min(kSmallBlocks, pow2_ceil((A.n + 256u - 1) / 256u));
   const uint32_t chunk = (A.n + blocks - 1) / blocks;
-  const uint32_t threads =
-      std::min(kSmallThreads, std::max((chunk + 127) / 128 * 128, std::min(R, 256u)));
   const uint32_t rounds = (chunk + threads - 1) / threads;
   const size_t smem = (3 + (size_t)threads / 32) * R * 4;
   MVR_CUDA(c, raise_smem_limit((const void*)plan_small_kernel<I>, smem));
@@ -446,18 +476,27 @@ int plan_small(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_
 }
 
 // One pass over the tiles; I: what it reads its keys from.
+template <class I, uint32_t ROUNDS>
+int plan_pass_of(Ctx* c, const PlanArgs& A, const void* kin, const uint32_t* vin, int shift, int bits, bool last,
+                 uint32_t* kout, uint32_t* vout, uint32_t* hist, uint32_t* sums) {
+  cudaStream_t st = c->stream;
+  constexpr uint32_t kTile = kTileThreads * ROUNDS;
+  const uint32_t tiles = (uint32_t)((A.n + (kTile - 1ull)) / kTile), R = 1u << bits;
+  const size_t smem = (2 * R + std::max(kTileThreads / 32 * R, 2 * kTile)) * 4;
+  const auto count = plan_hist_kernel<I, ROUNDS>;
+  MVR_CUDA(c, launch_pdl(count, tiles, kTileThreads, 0, st, kin, A.n, A.rows, shift, R, tiles, hist));
+  MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
+  const auto scatter = last ? plan_scatter_kernel<I, ROUNDS, true> : plan_scatter_kernel<I, ROUNDS, false>;
+  MVR_CUDA(c, raise_smem_limit((const void*)scatter, smem));
+  MVR_CUDA(c, launch_pdl(scatter, tiles, kTileThreads, smem, st, A, kin, vin, shift, bits, tiles, hist, sums, kout,
+                         vout));
+  return MVR_OK;
+}
 template <class I>
 int plan_pass(Ctx* c, const PlanArgs& A, const void* kin, const uint32_t* vin, int shift, int bits, bool last,
               uint32_t* kout, uint32_t* vout, uint32_t* hist, uint32_t* sums) {
-  cudaStream_t st = c->stream;
-  const uint32_t tiles = (uint32_t)((A.n + (kTile - 1ull)) / kTile), R = 1u << bits;
-  const size_t smem = (2 * R + std::max(kTileThreads / 32 * R, 2 * kTile)) * 4;
-  MVR_CUDA(c, launch_pdl(plan_hist_kernel<I>, tiles, kTileThreads, 0, st, kin, A.n, A.rows, shift, R, tiles, hist));
-  MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
-  const auto scatter = last ? plan_scatter_kernel<I, true> : plan_scatter_kernel<I, false>;
-  MVR_CUDA(c, raise_smem_limit((const void*)scatter, smem));
-  MVR_CUDA(c, launch_pdl(scatter, tiles, kTileThreads, smem, st, A, kin, vin, shift, bits, tiles, hist, sums, kout, vout));
-  return MVR_OK;
+  const auto pass = few_rounds(A.n) ? plan_pass_of<I, kFewRounds> : plan_pass_of<I, kManyRounds>;
+  return pass(c, A, kin, vin, shift, bits, last, kout, vout, hist, sums);
 }
 
 int plan_tiles(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_t* v0, uint32_t* k1, uint32_t* v1,
@@ -512,20 +551,18 @@ int mvr_token_plan_device(mvr_ctx* h, const void* d_ids, int id_bytes, uint64_t 
                                 d_offsets, d_order,  d_keys,          d_slot};
   const mvr::tok::PlanSpace ws(n_ids, rows);
   auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(d_workspace) + off); };
-  if (n_ids <= mvr::tok::kSmallMax) {
-    const mvr::tok::Digits D(rows, mvr::tok::kSmallBits);
+  const mvr::tok::Digits D(rows);
+  if (mvr::tok::is_small(n_ids, D)) {
     const auto small = id_bytes == 8 ? mvr::tok::plan_small<uint64_t> : mvr::tok::plan_small<uint32_t>;
     MVR_TRY(small(c, A, D, at(ws.k0), at(ws.v0), at(ws.k1), at(ws.v1)));
     if (D.passes == 1) return MVR_OK;  // the offsets came with the counts
   } else {
-    const mvr::tok::Digits D(rows, mvr::tok::kTileBits);
     MVR_TRY(mvr::tok::plan_tiles(c, A, D, at(ws.k0), at(ws.v0), at(ws.k1), at(ws.v1), at(ws.hist), at(ws.sums)));
   }
   // Walking the places costs one read each, a search some twenty dependent ones
   // a row: the walk is for rows that do not outnumber the places by far.
   if (rows <= 8 * n_ids)
-    MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_borders_kernel, (unsigned)(n_ids / mvr::tok::kBorderPlaces + 1),
-                                  256, 0, st, A));
+    MVR_TRY(mvr::tok::plan_borders(c, A));
   else
     MVR_CUDA(c, mvr::launch_pdl(mvr::tok::plan_offsets_kernel, (unsigned)(rows / 256 + 1), 256, 0, st, A));
   return MVR_OK;
