@@ -14,38 +14,49 @@ namespace {
 // the work is cut as for the lookup. With it a group of lanes has a row, for
 // the dot products.
 
-// dst[slot[i, c]] = w[i, c] * src[i]: a token's row is read once.
-template <class T, int V, int UR>
+// dst[slot[i, c]] = w[i, c] * src[i]: a token's row is read once. KU choices'
+// places are asked for at once, beside the rows.
+template <class T, int V, int UR, int KU>
 __global__ void __launch_bounds__(256)
 spread_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
               const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds) {
   const FlatBlock<UR> B(F);
-  uint64_t i[UR];
-  uint32_t c[UR];
+  src += B.row0 * ss;
+  slot += B.row0 * columns;
+  if (w) w += B.row0 * columns;
+  uint32_t i[UR], c[UR];
   Raw<T, V> x[UR];
 #pragma unroll
-  for (int j = 0; j < UR; ++j) {
-    if (B.at(j, &i[j], &c[j]))
-      x[j].load(src + i[j] * ss + (uint64_t)c[j] * V);
-    else
-      i[j] = ~0ull;
-  }
+  for (int j = 0; j < UR; ++j) B.place(j, &i[j], &c[j]);  // (0, 0) behind the end: read, not written
 #pragma unroll
-  for (int j = 0; j < UR; ++j) {
-    if (i[j] == ~0ull) continue;
-    for (uint32_t k = 0; k < columns; ++k) {
-      const uint32_t p = slot[i[j] * columns + k];
-      if (p >= pairs) continue;
-      Raw<T, V> r = x[j];
-      if (w) {
-        const float f = w[i[j] * columns + k];
-        float y[V];
+  for (int j = 0; j < UR; ++j) x[j].load(src + i[j] * ss + c[j] * V);
+  for (uint32_t k0 = 0; k0 < columns; k0 += KU) {
+    uint32_t p[UR][KU];
+    float f[UR][KU];
 #pragma unroll
-        for (int v = 0; v < V; ++v) y[v] = f * x[j].get(v);
-        r.set(y);
+    for (int j = 0; j < UR; ++j)
+#pragma unroll
+      for (int k = 0; k < KU; ++k)
+        p[j][k] = k0 + k < columns && B.in(j) ? slot[(uint64_t)i[j] * columns + k0 + k] : kNoSlot;
+    if (w)
+#pragma unroll
+      for (int j = 0; j < UR; ++j)
+#pragma unroll
+        for (int k = 0; k < KU; ++k) f[j][k] = p[j][k] < pairs ? w[(uint64_t)i[j] * columns + k0 + k] : 0.f;
+#pragma unroll
+    for (int j = 0; j < UR; ++j)
+#pragma unroll
+      for (int k = 0; k < KU; ++k) {
+        if (p[j][k] >= pairs) continue;
+        Raw<T, V> r = x[j];
+        if (w) {
+          float y[V];
+#pragma unroll
+          for (int v = 0; v < V; ++v) y[v] = f[j][k] * x[j].get(v);
+          r.set(y);
+        }
+        r.store(dst + p[j][k] * ds + c[j] * V);
       }
-      r.store(dst + p * ds + (uint64_t)c[j] * V);
-    }
   }
 }
 
@@ -55,9 +66,10 @@ __global__ void __launch_bounds__(256)
 collect_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
                const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds) {
   const FlatBlock<1> B(F);
-  uint64_t i;
-  uint32_t c;
-  if (!B.at(0, &i, &c)) return;
+  if (!B.in(0)) return;
+  uint32_t from, c;
+  B.place(0, &from, &c);
+  const uint64_t i = B.row0 + from;
   float acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.f;
@@ -160,28 +172,40 @@ collect_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint6
     f[k] = p[k] < pairs ? (w ? w[i * columns + k] : 1.f) : 0.f;
     dot[k] = 0.f;
   }
+  constexpr int U = KU <= 4 ? 2 : 1;  // chunks at once: eight rows' in flight
   if (i < n)
-    for (uint32_t c = l; c < chunks; c += L) {
-      Raw<T, V> o, x[KU];
-      o.load(other + i * other_s + (uint64_t)c * V);
-      float acc[V];
+    for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
+      Raw<T, V> o[U], x[U][KU];
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = 0.f;
+      for (int u = 0; u < U; ++u) {
+        const uint32_t c = c0 + u * L;
+        o[u].zero();
+        if (c < chunks) o[u].load(other + i * other_s + (uint64_t)c * V);
 #pragma unroll
-      for (int k = 0; k < KU; ++k) {
-        x[k].zero();
-        if (p[k] < pairs) x[k].load(src + p[k] * ss + (uint64_t)c * V);
+        for (int k = 0; k < KU; ++k) {
+          x[u][k].zero();
+          if (p[k] < pairs && c < chunks) x[u][k].load(src + p[k] * ss + (uint64_t)c * V);
+        }
       }
 #pragma unroll
-      for (int k = 0; k < KU; ++k)
+      for (int u = 0; u < U; ++u) {
+        const uint32_t c = c0 + u * L;
+        float acc[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float xv = x[k].get(v);
-          acc[v] = fmaf(f[k], xv, acc[v]);
-          dot[k] = fmaf(o.get(v), xv, dot[k]);
+        for (int v = 0; v < V; ++v) acc[v] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KU; ++k)
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float xv = x[u][k].get(v);
+            acc[v] = fmaf(f[k], xv, acc[v]);
+            dot[k] = fmaf(o[u].get(v), xv, dot[k]);
+          }
+        if (c < chunks) {
+          o[u].set(acc);
+          o[u].store(dst + i * ds + (uint64_t)c * V);
         }
-      o.set(acc);
-      o.store(dst + i * ds + (uint64_t)c * V);
+      }
     }
 #pragma unroll
   for (int k = 0; k < KU; ++k) {
@@ -210,12 +234,12 @@ int spread(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t
             L, chunks, (const T*)src, ss, columns, pairs, slot, w, (T*)dst, ds, (const T*)other, os, dw);
       } else {
         const Flat F = flat_of(n, chunks);
-        if (many(c, F))
-          spread_kernel<T, V, 4><<<blocks_of(F.total, 1024), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs,
-                                                                                  slot, w, (T*)dst, ds);
-        else
-          spread_kernel<T, V, 1><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs,
-                                                                                 slot, w, (T*)dst, ds);
+        const bool several = many(c, F);
+        const auto kernel = several ? (columns <= 2 ? spread_kernel<T, V, 4, 2> : spread_kernel<T, V, 2, 8>)
+                                    : (columns <= 2 ? spread_kernel<T, V, 1, 2> : spread_kernel<T, V, 1, 8>);
+        const int per = several ? (columns <= 2 ? 1024 : 512) : 256;
+        kernel<<<blocks_of(F.total, per), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs, slot, w, (T*)dst,
+                                                               ds);
       }
       MVR_CUDA(c, cudaGetLastError());
       return (int)MVR_OK;
@@ -242,20 +266,14 @@ int collect(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_
       if (dw && columns <= kDotColumns) {
         const uint32_t L = lanes_of(c, n, chunks);
         const unsigned blocks = blocks_of(n, 256 / L);
-        if (columns <= 2)
-          collect_dot_kernel<T, V, 2><<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w, (T*)dst,
-                                                                     ds, o, os, dw);
-        else
-          collect_dot_kernel<T, V, kDotColumns><<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w,
-                                                                               (T*)dst, ds, o, os, dw);
+        const auto kernel = columns <= 2   ? collect_dot_kernel<T, V, 2>
+                            : columns <= 4 ? collect_dot_kernel<T, V, 4>
+                                           : collect_dot_kernel<T, V, kDotColumns>;
+        kernel<<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w, (T*)dst, ds, o, os, dw);
       } else {
         const Flat F = flat_of(n, chunks);
-        if (columns <= 2)
-          collect_kernel<T, V, 2><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w,
-                                                                                  (T*)dst, ds);
-        else
-          collect_kernel<T, V, 8><<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w,
-                                                                                  (T*)dst, ds);
+        const auto kernel = columns <= 2 ? collect_kernel<T, V, 2> : collect_kernel<T, V, 4>;
+        kernel<<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w, (T*)dst, ds);
         if (dw) {  // the dots on their own: src once more
           const uint32_t L = lanes_of(c, pairs, chunks);
           spread_dot_kernel<T, V, false><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(

@@ -76,8 +76,8 @@ int lookup_run(Ctx* c, uint64_t n, uint32_t chunks, const void* table, uint64_t 
 // workspace to lookup_grad_join_kernel. Every sum's order is fixed by the
 // places, so results do not depend on which block runs first.
 
-// Chunks a lane holds: V elements of a row are at most 16 bytes; rows that
-// cannot be read 16 bytes at a time take several.
+// Chunks a lane holds: 16 bytes of a row, in several pieces where its length or
+// alignment does not allow one.
 template <class T, int V>
 constexpr int chunks_per_lane() {
   return (int)sizeof(T) * V >= 16 ? 1 : (int)sizeof(T) * V >= 8 ? 2 : 4;
@@ -174,24 +174,15 @@ struct GroupSums {
 
 // Places of a tile whose plan entries a block keeps in shared memory.
 constexpr uint32_t kMaxTile = 2048;
-constexpr int kFlight = 4;  // rows a lane takes at once, and as many on their way
+constexpr int kFlight = 4;  // rows a lane takes at once
 
-// Bytes of a row's chunks in a lane.
-template <class T, int V>
-constexpr int lane_bytes() {
-  return chunks_per_lane<T, V>() * (int)sizeof(T) * V;
-}
-template <class T, int V>
-size_t grad_smem(uint32_t tile) {
-  return (size_t)2 * kFlight * lane_bytes<T, V>() * 256 + (size_t)tile * 12;
-}
+size_t grad_smem(uint32_t tile) { return (size_t)tile * 12; }
 
 template <class T, class O, int V, bool DSCALE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 3)
 lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   constexpr int NCH = chunks_per_lane<T, V>();
   constexpr int U = kFlight;
-  constexpr uint32_t kRing = 2u * U * lane_bytes<T, V>() * 256;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float s_head[256 * NCH * V], s_tail[256 * NCH * V];
   __shared__ uint8_t s_hkind[256], s_has_tail[256];  // head: 0 none, 1 ends here, 2 goes on
@@ -215,7 +206,7 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   }
   if (tile0 >= valid) return;
   // the tile's plan: keys, tokens, scales
-  uint32_t* s_key = reinterpret_cast<uint32_t*>(smem + kRing);
+  uint32_t* s_key = reinterpret_cast<uint32_t*>(smem);
   uint32_t* s_tok = s_key + tile;
   float* s_scale = reinterpret_cast<float*>(s_tok + tile);
   const uint32_t here = (uint32_t)min((uint64_t)tile, valid - tile0);
@@ -250,7 +241,7 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   const bool from_before_tile = tile0 && A.keys[tile0 - 1] == A.keys[tile0];
   __syncthreads();
 
-  const uint32_t a = min(here, g * S.per_group), b = min(here, a + S.per_group);  // places in the tile
+  const uint32_t a = g * S.per_group, b = min(here, a + S.per_group);  // places in the tile: none where a >= b
   uint32_t col[NCH];
   bool on[NCH];
 #pragma unroll
@@ -278,55 +269,15 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
       for (int k = 0; k < NCH; ++k)
         if (on[k]) put_sum(A.dtable + (uint64_t)key * S.ds + col[k], acc[k], A.alpha, A.accumulate);
   };
-  // The ring: a lane copies and reads its own chunks only, so it waits for its
-  // own copies and for nobody else.
-  auto ring = [&](uint32_t slot, int u, int k) {
-    return reinterpret_cast<T*>(smem) + (((slot * U + u) * NCH + k) * 256 + threadIdx.x) * V;
-  };
-  auto fetch1 = [&](uint32_t t, uint32_t slot, int u) {
-    const T* row = A.grad + t * S.gs;
-#pragma unroll
-    for (int k = 0; k < NCH; ++k)
-      if (on[k]) {
-        if constexpr (sizeof(T) * V >= 4)
-          cp_async<(int)sizeof(T) * V>(ring(slot, u, k), row + col[k]);
-        else
-          *ring(slot, u, k) = row[col[k]];
-      }
-  };
-  auto fetch = [&](uint32_t p0, uint32_t slot) {
-    if (p0 + U <= b) {
-#pragma unroll
-      for (int u = 0; u < U; u += 4) {
-        const uint4 t = *reinterpret_cast<const uint4*>(s_tok + p0 + u);
-        fetch1(t.x, slot, u);
-        fetch1(t.y, slot, u + 1);
-        fetch1(t.z, slot, u + 2);
-        fetch1(t.w, slot, u + 3);
-      }
-    } else {
-#pragma unroll 1
-      for (int u = 0; p0 + u < b; ++u) fetch1(s_tok[p0 + u], slot, u);
-    }
-    cp_async_commit();
-  };
-
   bool started = a < b && (a ? s_key[a - 1] != s_key[a] : !from_before_tile);
   uint32_t cur = a < b ? s_key[a] : S.rows;
   uint32_t hkind = 0;
   Raw<T, V> trow[NCH];  // the table's row of `cur`
-  auto load_row = [&](Raw<T, V> (&r)[NCH], uint32_t key) {
+  auto load_row = [&](Raw<T, V> (&r)[NCH], const T* base, uint64_t at, bool in) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       r[k].zero();
-      if (key < S.rows && on[k]) r[k].load(A.table + key * S.ts + col[k]);
-    }
-  };
-  auto take = [&](Raw<T, V> (&r)[NCH], uint32_t slot, int u) {
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      r[k].zero();
-      if (on[k]) r[k].read(ring(slot, u, k));
+      if (in && on[k]) r[k].load(base + at + col[k]);
     }
   };
   auto add = [&](const Raw<T, V> (&r)[NCH], float f) {
@@ -343,65 +294,78 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
       for (int v = 0; v < V; ++v) d = fmaf(x[k].get(v), y[k].get(v), d);
     return d;
   };
-  fetch(a, 0);
-  if constexpr (DSCALE) load_row(trow, cur);
+  if constexpr (DSCALE) load_row(trow, A.table, cur * S.ts, cur < S.rows);
 
+  Raw<T, V> row[U][NCH];
+  float f[U];
+  auto load_step = [&](uint32_t p0) {  // groups begin at multiples of 8 places
+#pragma unroll
+    for (int u = 0; u < U; u += 4) {
+      if (p0 + u >= b) break;
+      const uint4 t = *reinterpret_cast<const uint4*>(s_tok + p0 + u);
+      load_row(row[u], A.grad, t.x * S.gs, true);
+      load_row(row[u + 1], A.grad, t.y * S.gs, p0 + u + 1 < b);
+      load_row(row[u + 2], A.grad, t.z * S.gs, p0 + u + 2 < b);
+      load_row(row[u + 3], A.grad, t.w * S.gs, p0 + u + 3 < b);
+      const float4 x = *reinterpret_cast<const float4*>(s_scale + p0 + u);
+      f[u] = x.x;
+      f[u + 1] = x.y;
+      f[u + 2] = x.z;
+      f[u + 3] = x.w;
+    }
+  };
+  load_step(a);
   const uint32_t steps = (S.per_group + U - 1) / U;  // the same for all lanes: exchanges inside
   for (uint32_t step = 0; step < steps; ++step) {
-    const uint32_t p0 = a + step * U, slot = step & 1;
+    const uint32_t p0 = a + step * U;
     if (__all_sync(0xffffffffu, p0 >= b)) break;
-    cp_async_wait<0>();
-    fetch(p0 + U, slot ^ 1);
     float dot[U];
     // sorted: all of them are of the current key when the last is
     if (p0 + U <= b && s_key[p0 + U - 1] == cur) {
 #pragma unroll
-      for (int u = 0; u < U; u += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(s_scale + p0 + u);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          Raw<T, V> row[NCH];
-          take(row, slot, u + q);
-          add(row, q == 0 ? f.x : q == 1 ? f.y : q == 2 ? f.z : f.w);
-          if constexpr (DSCALE) dot[u + q] = times(row, trow);
-        }
+      for (int u = 0; u < U; ++u) {
+        add(row[u], f[u]);
+        if constexpr (DSCALE) dot[u] = times(row[u], trow);
       }
     } else {
+      uint32_t begins = 0;  // bit u: place p0 + u begins a key
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p0 + u < b && s_key[p0 + u] != (u ? s_key[p0 + u - 1] : cur)) begins |= 1u << u;
       if constexpr (DSCALE) {
         Raw<T, V> other[U][NCH];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_row(other[u], p0 + u < b ? s_key[p0 + u] : S.rows);
-#pragma unroll
         for (int u = 0; u < U; ++u) {
-          dot[u] = 0.f;
-          if (p0 + u < b) {
-            Raw<T, V> row[NCH];
-            take(row, slot, u);
-            dot[u] = times(row, other[u]);
-          }
+          const uint32_t key = p0 + u < b ? s_key[p0 + u] : S.rows;
+          load_row(other[u], A.table, key * S.ts, key < S.rows);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) dot[u] = times(row[u], other[u]);
 #pragma unroll
         for (int k = 0; k < NCH; ++k) trow[k] = other[U - 1][k];  // of the last place's key
       }
-#pragma unroll 1
-      for (int u = 0; u < U && p0 + u < b; ++u) {
-        const uint32_t key = s_key[p0 + u];
-        if (key != cur) {
-          if (started) {
-            write(cur);
-          } else {
-            stage(s_head);
-            hkind = 1;
-          }
-          started = true;
-          clear();
-          cur = key;
+      const int count = min((uint32_t)U, b - min(b, p0));
+      // the places up to the next key's first, then that key
+      for (int from = 0;;) {
+        const int to = begins ? __ffs(begins) - 1 : count;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u >= from && u < to) add(row[u], f[u]);
+        if (!begins) break;
+        if (started) {
+          write(cur);
+        } else {
+          stage(s_head);
+          hkind = 1;
         }
-        Raw<T, V> row[NCH];
-        take(row, slot, u);
-        add(row, s_scale[p0 + u]);
+        started = true;
+        clear();
+        cur = s_key[p0 + to];
+        begins &= begins - 1;
+        from = to;
       }
     }
+    load_step(p0 + U);  // on their way during the exchanges
     if constexpr (DSCALE) {
       __syncwarp();
       const GroupSums<U> sums(dot, L, l);
@@ -466,11 +430,13 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
 }
 
 // Block t sums the key that crosses the border of tiles t and t + 1 and has
-// crossed no earlier one: what it left behind the tiles, in their order (the
-// warps take every eighth), then its end. W columns a lane.
+// crossed no earlier one: what it left behind the tiles, in their order, then
+// its end. L lanes have a tile's sums, W columns each, and the block's groups
+// of L lanes take every 512 / L-th tile.
+constexpr uint32_t kJoinThreads = 512;
 template <class O, int W>
-__global__ void __launch_bounds__(256)
-lookup_grad_join_kernel(GradShape S, uint32_t tile, const uint32_t* __restrict__ offsets,
+__global__ void __launch_bounds__(kJoinThreads)
+lookup_grad_join_kernel(GradShape S, uint32_t L, uint32_t tile, const uint32_t* __restrict__ offsets,
                         const uint32_t* __restrict__ keys, const float* __restrict__ part, O* __restrict__ dtable,
                         float alpha, int accumulate) {
   grid_dependency_wait();
@@ -479,9 +445,9 @@ lookup_grad_join_kernel(GradShape S, uint32_t tile, const uint32_t* __restrict__
   if (key >= S.rows || before != key) return;
   const uint32_t first = offsets[key] / tile, last = min((offsets[key + 1] - 1) / tile, S.tiles - 1);
   if (first != blockIdx.x) return;
-  __shared__ float s_sum[8][W][32];
-  const uint32_t w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  for (uint32_t c0 = blockIdx.y * (32 * W); c0 < S.dim; c0 += gridDim.y * (32 * W)) {
+  __shared__ float s_sum[W][kJoinThreads];
+  const uint32_t g = threadIdx.x / L, l = threadIdx.x & (L - 1), G = kJoinThreads / L;
+  for (uint32_t c0 = blockIdx.y * (L * W); c0 < S.dim; c0 += gridDim.y * (L * W)) {
     const uint32_t c = c0 + l * W;
     float acc[W];
     Raw<float, W> x;
@@ -489,23 +455,25 @@ lookup_grad_join_kernel(GradShape S, uint32_t tile, const uint32_t* __restrict__
     for (int v = 0; v < W; ++v) acc[v] = 0.f;
     if (c < S.dim) {
 #pragma unroll 4
-      for (uint32_t t = first + w; t < last; t += 8) {
+      for (uint32_t t = first + g; t < last; t += G) {
         x.load(part + ((uint64_t)t * 2 + 1) * S.dim + c);
 #pragma unroll
         for (int v = 0; v < W; ++v) acc[v] += x.get(v);
       }
     }
 #pragma unroll
-    for (int v = 0; v < W; ++v) s_sum[w][v][l] = acc[v];
+    for (int v = 0; v < W; ++v) s_sum[v][threadIdx.x] = acc[v];
     __syncthreads();
-    if (w == 0 && c < S.dim) {
+    if (g == 0 && c < S.dim) {
       x.load(part + (uint64_t)last * 2 * S.dim + c);
+      const uint32_t used = min(G, last - first);
+#pragma unroll 1
+      for (uint32_t q = 1; q < used; ++q)
+#pragma unroll
+        for (int v = 0; v < W; ++v) acc[v] += s_sum[v][q * L + l];
 #pragma unroll
       for (int v = 0; v < W; ++v) {
-#pragma unroll
-        for (int q = 1; q < 8; ++q) acc[v] += s_sum[q][v][l];
-        acc[v] += x.get(v);
-        const float sum[1] = {acc[v]};
+        const float sum[1] = {acc[v] + x.get(v)};
         put_sum<O, 1>(dtable + (uint64_t)key * S.ds + c + v, sum, alpha, accumulate);
       }
     }
@@ -579,14 +547,15 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
   if (S.tiles + S.fills == 0) return MVR_OK;
   const bool with_dscale = A.dscale && slabs == 1;
   const auto kernel = with_dscale ? lookup_grad_tile_kernel<T, O, V, true> : lookup_grad_tile_kernel<T, O, V, false>;
-  const size_t smem = grad_smem<T, V>(tile);
+  const size_t smem = grad_smem(tile);
   MVR_CUDA(c, raise_smem_limit((const void*)kernel, smem));
   MVR_CUDA(c, launch_pdl(kernel, dim3(S.fills + S.tiles, slabs), 256, smem, st, A));
   if (S.tiles > 1) {  // a block's columns once, while the grid stays small: most blocks have nothing to join
-    const uint32_t w = S.dim % 4 == 0 ? 4 : 1, columns = (S.dim + 32 * w - 1) / (32 * w);
+    const uint32_t w = S.dim % 4 == 0 ? 4 : 1, L = std::min(32u, pow2_ceil(S.dim / w));
+    const uint32_t columns = (S.dim + L * w - 1) / (L * w);
     const dim3 grid(S.tiles - 1, std::max(1u, std::min(columns, 32768u / S.tiles)));
     const auto join = w == 4 ? lookup_grad_join_kernel<O, 4> : lookup_grad_join_kernel<O, 1>;
-    MVR_CUDA(c, launch_pdl(join, grid, 256, 0, st, S, tile, A.offsets, A.keys, A.part, A.dtable, A.alpha,
+    MVR_CUDA(c, launch_pdl(join, grid, kJoinThreads, 0, st, S, L, tile, A.offsets, A.keys, A.part, A.dtable, A.alpha,
                            A.accumulate));
   }
   if (A.dscale && S.tiles && !with_dscale) {  // a row's parts lie in several blocks

@@ -187,16 +187,6 @@ struct FlatBlock {
     *row = in(j) ? q : 0;
     *chunk = in(j) ? x - q * F.chunks : 0;
   }
-  // false behind the end
-  __device__ __forceinline__ bool at(int j, uint64_t* row, uint32_t* chunk) const {
-    const uint32_t local = j * 256 + threadIdx.x;
-    if (first + local >= F.total) return false;
-    const uint32_t x = rem0 + local;
-    const uint32_t q = F.shift >= 0 ? x >> F.shift : x / F.chunks;
-    *row = row0 + q;
-    *chunk = x - q * F.chunks;
-    return true;
-  }
 };
 
 inline size_t elem_size(int dtype) { return dtype == MVR_F32 ? 4 : 2; }
@@ -234,12 +224,12 @@ inline Flat flat_of(uint64_t n, uint32_t chunks) {
 // Four elements a thread when that still fills every SM with threads.
 inline bool many(Ctx* c, const Flat& F) { return F.total >= 4ull * 2048 * c->sm_count; }
 
-// Lanes of a row for the dot products: one chunk a lane when there are few
-// rows; as many as four a lane (fewer lanes to sum over) while every SM keeps
-// 1024 threads.
+// Lanes of a row for the dot products: as few as sixteen chunks a lane leave (the
+// exchanges between lanes cost more than the loop), while every SM keeps 1024
+// threads.
 inline uint32_t lanes_of(Ctx* c, uint64_t n, uint32_t chunks) {
   uint32_t L = std::min(256u, pow2_ceil(chunks));
-  while (L > 1 && chunks < 4 * L && n * (L / 2) >= 1024ull * c->sm_count) L /= 2;
+  while (L > 1 && chunks < 16 * L && n * (L / 2) >= 1024ull * c->sm_count) L /= 2;
   return L;
 }
 

@@ -22,7 +22,7 @@ constexpr int kMostBits = 10;  // of a digit
 constexpr uint32_t kSmallThreads = 256, kSmallRounds = 8, kSmallBlocks = 8;
 constexpr uint32_t kSmallMax = kSmallThreads * kSmallRounds * kSmallBlocks;  // 16,384 pairs
 constexpr uint32_t kSmallMaxPasses = kSmallMax / 2;                          // where one pass is not enough
-constexpr uint32_t kTileThreads = 512;
+constexpr uint32_t kTileThreads = 256;
 
 struct PlanArgs {
   const void* ids;
@@ -255,10 +255,11 @@ plan_scan_kernel(uint32_t tiles, uint32_t* __restrict__ hist, uint32_t* __restri
 }
 
 // A tile's pairs, sorted by digit in shared memory first so that each digit's
-// run is written in one piece. 42 registers a thread let three blocks share an
-// SM, so that up to 1.8 million pairs are one wave of blocks.
+// run is written in one piece. At 1,521,797 pairs blocks of 256 threads that
+// share an SM by fours measured best (the plan 51 us; 54 with six or with
+// blocks of 512 threads by twos, 70 with one of 1024).
 template <class I, uint32_t ROUNDS, bool LAST>
-__global__ void __launch_bounds__(kTileThreads, 3)
+__global__ void __launch_bounds__(kTileThreads, 4)
 plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __restrict__ vin, int shift,
                     int bits, uint32_t tiles, const uint32_t* __restrict__ hist,
                     const uint32_t* __restrict__ total, uint32_t* __restrict__ kout, uint32_t* __restrict__ vout) {
@@ -423,10 +424,9 @@ struct Digits {
 // launches at some 10,000 pairs.
 bool is_small(uint64_t n, const Digits& D) { return n <= (D.passes == 1 ? kSmallMax : kSmallMaxPasses); }
 
-// Pairs a thread of a tile: few while that gives more blocks than share the
-// SMs at once.
-constexpr uint64_t kFewRounds = 2, kManyRounds = 8;
-bool few_rounds(uint64_t n) { return n <= 444 * kFewRounds * kTileThreads; }
+// Pairs a thread of a tile: few until the blocks are more than share the SMs.
+constexpr uint32_t kFewRounds = 4, kManyRounds = 8;
+bool few_rounds(uint64_t n) { return n <= 148ull * 4 * kFewRounds * kTileThreads; }
 
 // Workspace: two sets of pairs for the passes, and the counts of the tiles.
 struct PlanSpace {

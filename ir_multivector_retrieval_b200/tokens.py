@@ -14,7 +14,11 @@ waiting; they may be captured into a CUDA graph. There is no CPU fallback.
 """
 from __future__ import annotations
 
+import atexit
 import ctypes as C
+import functools
+import threading
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 from . import _lib
@@ -27,58 +31,59 @@ def _refuse(msg: str, name: str = "InvalidArgument"):
     raise MvrError(CODES[name], msg)
 
 
+@functools.cache
 def _torch():
     import torch
 
     return torch
 
 
-_types: dict = {}
+@functools.cache
+def _types() -> dict:
+    """Element types (mvr_dtype) and id types (bytes) by torch type."""
+    torch = _torch()
+    return {"rows": {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2},
+            "ids": {torch.int32: 4, torch.uint32: 4, torch.int64: 8}, "f32": torch.float32, "i32": torch.int32}
 
 
 def _dtype(t, what: str) -> int:
-    if not _types:
-        torch = _torch()
-        _types.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-    d = _types.get(t.dtype)
+    d = _types()["rows"].get(getattr(t, "dtype", None))
     if d is None:
-        _refuse(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+        _refuse(f"{what} must be a float32, bfloat16 or float16 tensor, not {getattr(t, 'dtype', type(t))}")
     return d
 
 
-def _is_device(t) -> bool:
-    return hasattr(t, "is_cuda") and t.is_cuda
-
-
 def _id_bytes(ids) -> int:
-    torch = _torch()
-    if ids.dtype in (torch.int32, torch.uint32):
-        return 4
-    if ids.dtype == torch.int64:
-        return 8
-    _refuse(f"ids must be int32, int64 or uint32, not {ids.dtype}")
+    n = _types()["ids"].get(getattr(ids, "dtype", None))
+    if n is None:
+        _refuse(f"ids must be an int32, int64 or uint32 tensor, not {getattr(ids, 'dtype', type(ids))}")
+    return n
 
 
 def _rows(t, what: str, n: int | None = None, dim: int | None = None):
-    """`t` as a 2-D view (copied where its rows are not consecutive) and its
-    row stride."""
-    if t.dim() < 2:
-        _refuse(f"{what} must have rows: at least two dimensions", "DimMismatch")
-    if t.dim() > 2:
+    """`t` as a 2-D view (copied where its rows are not consecutive), its row
+    length and its row stride."""
+    if t.dim() != 2:
+        if t.dim() < 2:
+            _refuse(f"{what} must have rows: at least two dimensions", "DimMismatch")
         t = t.reshape(-1, t.shape[-1])
-    if dim is not None and t.shape[1] != dim:
-        _refuse(f"{what} has rows of {t.shape[1]}, not {dim}", "DimMismatch")
-    if n is not None and t.shape[0] != n:
-        _refuse(f"{what} has {t.shape[0]} rows, not {n}", "LengthMismatch")
-    if t.shape[1] == 0:
+    m, d = t.shape
+    if dim is not None and d != dim:
+        _refuse(f"{what} has rows of {d}, not {dim}", "DimMismatch")
+    if n is not None and m != n:
+        _refuse(f"{what} has {m} rows, not {n}", "LengthMismatch")
+    if d == 0:
         _refuse(f"{what} has rows of length 0", "DimMismatch")
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < 0:
+    stride, one = t.stride()
+    if one != 1 and d > 1:
         t = t.contiguous()
-    return t, t.stride(0)
+        stride = d
+    return t, d, stride
 
 
 def _out_rows(t, what: str, n: int, dim: int, dtype):
-    """An output given by the caller: written in place, so never copied."""
+    """Address and row stride of an output given by the caller: written in
+    place, so never copied."""
     if t.dtype != dtype:
         _refuse(f"{what} must be {dtype}, not {t.dtype}")
     if t.dim() < 2 or t.shape[-1] != dim:
@@ -90,83 +95,123 @@ def _out_rows(t, what: str, n: int, dim: int, dtype):
             t = t.view(n, dim)
         except RuntimeError:
             _refuse(f"{what} must be viewable as {n} rows")
-    if dim > 1 and t.stride(1) != 1 or n > 1 and t.stride(0) < dim:
+    stride, one = t.stride()
+    if dim > 1 and one != 1 or n > 1 and stride < dim:
         _refuse(f"{what} must have consecutive, separate rows")
-    return t, t.stride(0) if n > 1 else max(t.stride(0), dim)
+    return t.data_ptr(), stride if n > 1 else max(stride, dim)
 
 
 def _f32(t, n: int, what: str):
-    if t is None:
-        return None
-    if t.dtype != _torch().float32:
+    if t.dtype != _types()["f32"]:
         _refuse(f"{what} must be float32, not {t.dtype}")
     if t.numel() != n:
         _refuse(f"{what} has {t.numel()} values, not {n}", "LengthMismatch")
     return t if t.is_contiguous() else t.contiguous()
 
 
-class _Call:
-    """One call's context and stream: tensors checked to lie on the context's
-    GPU, the context switched to the stream for the calls made inside."""
+@functools.cache
+def _raw_stream():
+    torch = _torch()
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda device: torch.cuda.current_stream(device).cuda_stream)
 
-    __slots__ = ("ctx", "handle", "lib", "own", "scope", "tensors")
 
-    def __init__(self, ctx, tensors):
-        dev = None
-        for t in tensors:
-            if t is None:
-                continue
-            if not _is_device(t):
-                _refuse("all tensors must be CUDA tensors (there is no CPU fallback)")
-            if dev is None:
-                dev = t.device
-            elif t.device != dev:
-                _refuse(f"tensors on {dev} and {t.device}")
-        if ctx is None:
-            ctx = _lib.default_context(dev.index)
-        elif ctx.device != dev.index:
-            _refuse(f"tensors on {dev}, context on device {ctx.device}")
-        self.ctx, self.handle, self.lib = ctx, ctx.handle, ctx.lib
-        self.tensors = tensors
-        self.own = self.scope = None
+def _stream_of(device: int) -> int:
+    """Handle of torch's current stream; 1 names the legacy default stream,
+    whose own handle, 0, would select a context's own stream."""
+    return _raw_stream()(device) or 1
 
-    def __enter__(self):
-        ctx = self.ctx
-        torch = _torch()
-        ctx.lock.acquire()
+
+class _Follower:
+    """A context of its own for each GPU, for calls that name none: its stream
+    is the one torch used at the last call, so that it is only set anew when
+    that changes."""
+
+    def __init__(self, device: int):
+        self.ctx = _lib.Context(device)
+        self.at = None
+
+
+_followers: dict = {}
+_followers_lock = threading.Lock()
+
+
+@atexit.register
+def _let_go():
+    # a context waits for its stream when it ends, and a stream of the
+    # program's may be gone by then
+    for f in _followers.values():
+        f.ctx.lib.mvr_ctx_set_stream(f.ctx.handle, None)
+
+
+def _follower(device: int) -> _Follower:
+    f = _followers.get(device)
+    if f is None:
+        with _followers_lock:
+            f = _followers.get(device)
+            if f is None:
+                f = _followers[device] = _Follower(device)
+    return f
+
+
+def _run(ctx, device: int, call):
+    """`call(lib, handle)` on the right context and stream, its status checked.
+    Contexts are not for two calls at once, hence the locks."""
+    if ctx is None:
+        f = _follower(device)
+        ctx = f.ctx
+        with ctx.lock:
+            here = _stream_of(device)
+            if f.at != here:
+                ctx.lib.mvr_ctx_set_stream(ctx.handle, here)
+                f.at = here
+            status = call(ctx.lib, ctx.handle)
+            if status:
+                ctx.check(status)
+        return
+    if ctx.device != device:
+        _refuse(f"tensors on device {device}, context on device {ctx.device}")
+    with ctx.lock:
+        here = _stream_of(device)
+        own = ctx.stream == 0
+        if own:
+            ctx.lib.mvr_ctx_set_stream(ctx.handle, here)
         try:
-            here = torch.cuda.current_stream(ctx.device).cuda_stream
-            if ctx.stream == 0:
-                # handle 0 would select the context's own stream: 1 names the legacy default stream
-                self.own = here or 1
-                self.lib.mvr_ctx_set_stream(self.handle, self.own)
-            elif ctx.stream != here and not (ctx.stream == 1 and here == 0):
-                # results come from the memory pool of the stream that writes
-                # them, and inputs stay alive for it
-                s = torch.cuda.ExternalStream(ctx.stream, device=ctx.device)
-                for t in self.tensors:
-                    if t is not None:
-                        t.record_stream(s)
-                self.scope = torch.cuda.stream(s)
-                self.scope.__enter__()
-        except BaseException:
-            ctx.lock.release()
-            raise
-        return self
-
-    def __exit__(self, *exc):
-        try:
-            if self.scope is not None:
-                self.scope.__exit__(*exc)
-            if self.own is not None:
-                self.lib.mvr_ctx_set_stream(self.handle, None)
+            status = call(ctx.lib, ctx.handle)
+            if status:
+                ctx.check(status)
         finally:
-            self.ctx.lock.release()
-        return False
+            if own:
+                ctx.lib.mvr_ctx_set_stream(ctx.handle, None)
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _place(ctx, *tensors):
+    """The GPU that all the tensors lie on, and the scope in which results and
+    copies are made: nothing to do on torch's current stream. With a stream
+    given to ``ctx.set_stream`` they come from that stream's memory pool, and
+    the inputs stay alive for it."""
+    device = -1
+    for t in tensors:
+        if t is None:
+            continue
+        if not getattr(t, "is_cuda", False):
+            _refuse("all tensors must be CUDA tensors (there is no CPU fallback)")
+        d = t.get_device()
+        if device < 0:
+            device = d
+        elif d != device:
+            _refuse(f"tensors on devices {device} and {d}")
+    if ctx is None or ctx.stream == 0 or ctx.stream == _stream_of(device):
+        return device, _here
+    torch = _torch()
+    s = torch.cuda.ExternalStream(ctx.stream, device=device)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(s)
+    return device, torch.cuda.stream(s)
+
+
+_here = nullcontext()
 
 
 @dataclass
@@ -198,43 +243,68 @@ class Plan:
         return self.slot.numel() // s[-1] if len(s) > 1 and s[-1] else s[0] if len(s) == 1 else 0
 
     def _check(self):
-        torch = _torch()
-        for name in ("offsets", "order", "keys", "slot"):
-            t = getattr(self, name)
-            if t.dtype != torch.int32 or not t.is_contiguous():
-                _refuse(f"plan.{name} must be a contiguous int32 tensor")
-        if self.offsets.numel() != self.rows + 1 or not self.order.numel() == self.keys.numel() == self.slot.numel():
+        i32 = _types()["i32"]
+        for t in (self.offsets, self.order, self.keys, self.slot):
+            if t.dtype != i32 or not t.is_contiguous():
+                _refuse("a plan's tensors must be contiguous int32 tensors")
+        n = self.slot.numel()
+        if self.offsets.numel() != self.rows + 1 or self.order.numel() != n or self.keys.numel() != n:
             _refuse("plan: sizes differ", "LengthMismatch")
-        return self
+        return n
+
+
+@functools.lru_cache(maxsize=256)
+def _plan_bytes(n: int, rows: int) -> int:
+    need = C.c_uint64(0)
+    st = _lib.load().mvr_token_plan_bytes(n, rows, C.byref(need))
+    if st:
+        raise MvrError(st, "token_plan_bytes")
+    return need.value
+
+
+@functools.lru_cache(maxsize=256)
+def _grad_bytes(n: int, dim: int) -> int:
+    need = C.c_uint64(0)
+    st = _lib.load().mvr_lookup_grad_bytes(n, dim, C.byref(need))
+    if st:
+        raise MvrError(st, "lookup_grad_bytes")
+    return need.value
+
+
+def _workspace(like, need: int):
+    return like.new_empty(need, dtype=_torch().uint8) if need else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def plan(ids, rows: int, *, ctx=None) -> Plan:
     """Sort the ids ([n] or [n, columns]) by value, stable."""
-    torch = _torch()
     rows = int(rows)
     if not 0 < rows < MAX_IDS:
         _refuse(f"rows must be in [1, 2^31 - 2], not {rows}")
-    if not hasattr(ids, "dim") or ids.dim() not in (1, 2):
-        _refuse("ids must be a tensor of one or two dimensions")
+    idb = _id_bytes(ids)
+    if ids.dim() not in (1, 2):
+        _refuse("ids must have one or two dimensions")
     if ids.dim() == 2 and ids.shape[1] == 0:
         _refuse("ids have no columns")
-    idb = _id_bytes(ids)
     n = ids.numel()
     if n > MAX_IDS:
         _refuse("more than 2^31 - 1 ids")
-    with _Call(ctx, (ids,)) as c:
+    device, scope = _place(ctx, ids)
+    with scope:
         ids = ids.contiguous()
-        dev = ids.device
-        need = C.c_uint64(0)
-        c.ctx.check(c.lib.mvr_token_plan_bytes(n, rows, C.byref(need)), "token_plan_bytes")
-        offsets = torch.empty(rows + 1, dtype=torch.int32, device=dev)
-        order = torch.empty(n, dtype=torch.int32, device=dev)
-        keys = torch.empty(n, dtype=torch.int32, device=dev)
-        slot = torch.empty(ids.shape, dtype=torch.int32, device=dev)
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        c.ctx.check(c.lib.mvr_token_plan_device(c.handle, ids.data_ptr(), idb, n, rows, offsets.data_ptr(),
-                                                order.data_ptr(), keys.data_ptr(), slot.data_ptr(), ws.data_ptr(),
-                                                need.value), "token_plan")
+        i32 = _types()["i32"]
+        offsets = ids.new_empty(rows + 1, dtype=i32)
+        order = ids.new_empty(n, dtype=i32)
+        keys = ids.new_empty(n, dtype=i32)
+        slot = ids.new_empty(ids.shape, dtype=i32)
+        need = _plan_bytes(n, rows)
+        ws = _workspace(ids, need)
+        _run(ctx, device, lambda lib, h: lib.mvr_token_plan_device(
+            h, ids.data_ptr(), idb, n, rows, offsets.data_ptr(), order.data_ptr(), keys.data_ptr(), slot.data_ptr(),
+            _ptr(ws), need))
     return Plan(rows, offsets, order, keys, slot)
 
 
@@ -242,27 +312,26 @@ def lookup(table, ids, *, scale=None, alpha: float = 1.0, out=None, ctx=None):
     """``out[i] = (alpha * scale[i]) * table[ids[i]]``: the ids' shape plus the
     table's row length, in the table's type; zero rows where an id names none.
     ``scale`` (the ids' shape, f32) and ``out`` are optional."""
-    torch = _torch()
     dt = _dtype(table, "table")
     idb = _id_bytes(ids)
     n = ids.numel()
     if table.dim() != 2:
         _refuse("table must have two dimensions", "DimMismatch")
-    with _Call(ctx, (table, ids, scale, out)) as c:
-        table, ts = _rows(table, "table")
-        rows, dim = table.shape
-        ids = ids.contiguous()
-        scale = _f32(scale, n, "scale")
+    device, scope = _place(ctx, table, ids, scale, out)
+    with scope:
+        rows = table.shape[0]
+        t, dim, ts = _rows(table, "table")
+        ids_ = ids.contiguous()
+        if scale is not None:
+            scale = _f32(scale, n, "scale")
         if out is None:
-            res = torch.empty((*ids.shape, dim), dtype=table.dtype, device=table.device)
-            ptr_out, so = res.data_ptr(), dim
+            out = t.new_empty((*ids.shape, dim))
+            po, so = out.data_ptr(), dim
         else:
-            res = out
-            o, so = _out_rows(out, "out", n, dim, table.dtype)
-            ptr_out = o.data_ptr()
-        c.ctx.check(c.lib.mvr_lookup_device(c.handle, table.data_ptr(), dt, rows, dim, ts, ids.data_ptr(), idb, n,
-                                            _ptr(scale), alpha, ptr_out, so), "lookup")
-    return res
+            po, so = _out_rows(out, "out", n, dim, t.dtype)
+        _run(ctx, device, lambda lib, h: lib.mvr_lookup_device(
+            h, t.data_ptr(), dt, rows, dim, ts, ids_.data_ptr(), idb, n, _ptr(scale), alpha, po, so))
+    return out
 
 
 def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None, out=None, accumulate: bool = False,
@@ -274,110 +343,105 @@ def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None,
     table[ids[i]]>`` as the second of a pair. ``out`` (grad's type or f32)
     receives the first; with ``accumulate`` the sums are added to it and rows
     without an id are not touched."""
-    torch = _torch()
     dt = _dtype(grad, "grad")
-    plan._check()
-    n = plan.n_ids
+    n = plan._check()
+    rows = plan.rows
     if accumulate and out is None:
         _refuse("accumulate needs out")
-    with _Call(ctx, (grad, plan.offsets, plan.order, plan.keys, plan.slot, scale, table, out)) as c:
-        grad, gs = _rows(grad, "grad", n)
-        dim = grad.shape[1]
-        scale = _f32(scale, n, "scale")
-        dev = grad.device
+    device, scope = _place(ctx, grad, plan.offsets, plan.order, plan.keys, plan.slot, scale, table, out)
+    with scope:
+        g, dim, gs = _rows(grad, "grad", n)
+        if scale is not None:
+            scale = _f32(scale, n, "scale")
         tp, ts, dscale = None, dim, None
         if table is not None:
-            if table.dtype != grad.dtype:
-                _refuse(f"table is {table.dtype}, grad {grad.dtype}")
-            table, ts = _rows(table, "table", plan.rows, dim)
+            if table.dtype != g.dtype:
+                _refuse(f"table is {table.dtype}, grad {g.dtype}")
+            table, _, ts = _rows(table, "table", rows, dim)
             tp = table.data_ptr()
-            dscale = torch.empty(plan.slot.shape, dtype=torch.float32, device=dev)
+            dscale = g.new_empty(plan.slot.shape, dtype=_types()["f32"])
         if out is None:
-            res = torch.empty((plan.rows, dim), dtype=grad.dtype, device=dev)
-            po, so, odt = res.data_ptr(), dim, dt
+            out = g.new_empty((rows, dim))
+            po, so, odt = out.data_ptr(), dim, dt
         else:
-            res = out
             odt = _dtype(out, "out")
             if odt not in (dt, 0):
                 _refuse("out must have grad's type or float32")
-            o, so = _out_rows(out, "out", plan.rows, dim, out.dtype)
-            po = o.data_ptr()
-        need = C.c_uint64(0)
-        c.ctx.check(c.lib.mvr_lookup_grad_bytes(n, dim, C.byref(need)), "lookup_grad_bytes")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        c.ctx.check(c.lib.mvr_lookup_grad_device(
-            c.handle, grad.data_ptr(), dt, gs, n, plan.rows, dim, plan.offsets.data_ptr(), plan.order.data_ptr(),
+            po, so = _out_rows(out, "out", rows, dim, out.dtype)
+        need = _grad_bytes(n, dim)
+        ws = _workspace(g, need)
+        _run(ctx, device, lambda lib, h: lib.mvr_lookup_grad_device(
+            h, g.data_ptr(), dt, gs, n, rows, dim, plan.offsets.data_ptr(), plan.order.data_ptr(),
             plan.keys.data_ptr(), plan.slot.data_ptr(), _ptr(scale), alpha, tp, ts, po, odt, so, int(accumulate),
-            _ptr(dscale), ws.data_ptr(), need.value), "lookup_grad")
-    return res if table is None else (res, dscale)
+            _ptr(dscale), _ptr(ws), need))
+    return out if dscale is None else (out, dscale)
 
 
-def _weights(weights, plan: Plan):
-    return _f32(weights, plan.n_ids, "weights")
+def _token_call(name: str, src, what: str, from_n: int, plan: Plan, weights, to_n: int, out, ctx):
+    """group and ungroup: rows of `src` to rows of `out`."""
+    dt = _dtype(src, what)
+    n_ids = plan._check()
+    device, scope = _place(ctx, src, plan.slot, weights, out)
+    with scope:
+        s, dim, ss = _rows(src, what, from_n)
+        if weights is not None:
+            weights = _f32(weights, n_ids, "weights")
+        if out is None:
+            out = s.new_empty((to_n, dim))
+            po, so = out.data_ptr(), dim
+        else:
+            po, so = _out_rows(out, "out", to_n, dim, s.dtype)
+        _run(ctx, device, lambda lib, h: getattr(lib, name)(
+            h, s.data_ptr(), dt, ss, plan.n, plan.columns, dim, plan.slot.data_ptr(), _ptr(weights), po, so))
+    return out
+
+
+def _token_grad(name: str, src, from_n: int, plan: Plan, weights, other, other_what: str, other_n: int, to_n: int,
+                out, ctx):
+    """Their gradients: also the weights' where the forward rows are given."""
+    dt = _dtype(src, "dout")
+    n_ids = plan._check()
+    device, scope = _place(ctx, src, plan.slot, weights, other, out)
+    with scope:
+        s, dim, ss = _rows(src, "dout", from_n)
+        if weights is not None:
+            weights = _f32(weights, n_ids, "weights")
+        dw, op, os_ = None, None, dim
+        if other is not None:
+            if other.dtype != s.dtype:
+                _refuse(f"{other_what} is {other.dtype}, dout {s.dtype}")
+            other, _, os_ = _rows(other, other_what, other_n, dim)
+            op = other.data_ptr()
+            dw = s.new_empty(plan.slot.shape, dtype=_types()["f32"])
+        if out is None:
+            out = s.new_empty((to_n, dim))
+            po, so = out.data_ptr(), dim
+        else:
+            po, so = _out_rows(out, "out", to_n, dim, s.dtype)
+        _run(ctx, device, lambda lib, h: getattr(lib, name)(
+            h, s.data_ptr(), dt, ss, plan.n, plan.columns, dim, plan.slot.data_ptr(), _ptr(weights), op, os_, po, so,
+            _ptr(dw)))
+    return out if dw is None else (out, dw)
 
 
 def group(x, plan: Plan, *, weights=None, out=None, ctx=None):
     """The rows of x (one a token) in sorted order: ``out[slot[i, c]] =
     weights[i, c] * x[i]``, n * columns rows. Rows behind the last sorted one
     keep what ``out`` held (without ``out`` they are undefined)."""
-    torch = _torch()
-    dt = _dtype(x, "x")
-    plan._check()
-    with _Call(ctx, (x, plan.slot, weights, out)) as c:
-        x, xst = _rows(x, "x", plan.n)
-        dim = x.shape[1]
-        weights = _weights(weights, plan)
-        if out is None:
-            out = torch.empty((plan.n_ids, dim), dtype=x.dtype, device=x.device)
-        o, so = _out_rows(out, "out", plan.n_ids, dim, x.dtype)
-        c.ctx.check(c.lib.mvr_group_rows_device(c.handle, x.data_ptr(), dt, xst, plan.n, plan.columns, dim,
-                                                plan.slot.data_ptr(), _ptr(weights), o.data_ptr(), so), "group")
-    return out
+    return _token_call("mvr_group_rows_device", x, "x", plan.n, plan, weights, plan.n_ids, out, ctx)
 
 
 def group_grad(dout, plan: Plan, *, weights=None, x=None, out=None, ctx=None):
     """Gradients of ``group`` from that of its output: ``dx[i] = sum_c
     weights[i, c] * dout[slot[i, c]]`` and, where ``x`` is given, also that of
     the weights, ``<x[i], dout[slot[i, c]]>``, as the second of a pair."""
-    torch = _torch()
-    dt = _dtype(dout, "dout")
-    plan._check()
-    with _Call(ctx, (dout, plan.slot, weights, x, out)) as c:
-        dout, ds = _rows(dout, "dout", plan.n_ids)
-        dim = dout.shape[1]
-        weights = _weights(weights, plan)
-        dw, xp, xst = None, None, dim
-        if x is not None:
-            if x.dtype != dout.dtype:
-                _refuse(f"x is {x.dtype}, dout {dout.dtype}")
-            x, xst = _rows(x, "x", plan.n, dim)
-            xp = x.data_ptr()
-            dw = torch.empty(plan.slot.shape, dtype=torch.float32, device=dout.device)
-        if out is None:
-            out = torch.empty((plan.n, dim), dtype=dout.dtype, device=dout.device)
-        o, so = _out_rows(out, "out", plan.n, dim, dout.dtype)
-        c.ctx.check(c.lib.mvr_group_rows_grad_device(c.handle, dout.data_ptr(), dt, ds, plan.n, plan.columns, dim,
-                                                     plan.slot.data_ptr(), _ptr(weights), xp, xst, o.data_ptr(), so,
-                                                     _ptr(dw)), "group_grad")
-    return out if x is None else (out, dw)
+    return _token_grad("mvr_group_rows_grad_device", dout, plan.n_ids, plan, weights, x, "x", plan.n, plan.n, out, ctx)
 
 
 def ungroup(xs, plan: Plan, *, weights=None, out=None, ctx=None):
     """Sorted rows back to their tokens: ``out[i] = sum_c weights[i, c] *
     xs[slot[i, c]]``; zeros for a token none of whose ids names a row."""
-    torch = _torch()
-    dt = _dtype(xs, "xs")
-    plan._check()
-    with _Call(ctx, (xs, plan.slot, weights, out)) as c:
-        xs, st = _rows(xs, "xs", plan.n_ids)
-        dim = xs.shape[1]
-        weights = _weights(weights, plan)
-        if out is None:
-            out = torch.empty((plan.n, dim), dtype=xs.dtype, device=xs.device)
-        o, so = _out_rows(out, "out", plan.n, dim, xs.dtype)
-        c.ctx.check(c.lib.mvr_ungroup_rows_device(c.handle, xs.data_ptr(), dt, st, plan.n, plan.columns, dim,
-                                                  plan.slot.data_ptr(), _ptr(weights), o.data_ptr(), so), "ungroup")
-    return out
+    return _token_call("mvr_ungroup_rows_device", xs, "xs", plan.n_ids, plan, weights, plan.n, out, ctx)
 
 
 def ungroup_grad(dout, plan: Plan, *, weights=None, xs=None, out=None, ctx=None):
@@ -385,27 +449,8 @@ def ungroup_grad(dout, plan: Plan, *, weights=None, xs=None, out=None, ctx=None)
     weights[i, c] * dout[i]`` (rows behind the last sorted one keep what
     ``out`` held) and, where ``xs`` is given, also that of the weights,
     ``<dout[i], xs[slot[i, c]]>``, as the second of a pair."""
-    torch = _torch()
-    dt = _dtype(dout, "dout")
-    plan._check()
-    with _Call(ctx, (dout, plan.slot, weights, xs, out)) as c:
-        dout, ds = _rows(dout, "dout", plan.n)
-        dim = dout.shape[1]
-        weights = _weights(weights, plan)
-        dw, xp, xst = None, None, dim
-        if xs is not None:
-            if xs.dtype != dout.dtype:
-                _refuse(f"xs is {xs.dtype}, dout {dout.dtype}")
-            xs, xst = _rows(xs, "xs", plan.n_ids, dim)
-            xp = xs.data_ptr()
-            dw = torch.empty(plan.slot.shape, dtype=torch.float32, device=dout.device)
-        if out is None:
-            out = torch.empty((plan.n_ids, dim), dtype=dout.dtype, device=dout.device)
-        o, so = _out_rows(out, "out", plan.n_ids, dim, dout.dtype)
-        c.ctx.check(c.lib.mvr_ungroup_rows_grad_device(c.handle, dout.data_ptr(), dt, ds, plan.n, plan.columns, dim,
-                                                       plan.slot.data_ptr(), _ptr(weights), xp, xst, o.data_ptr(), so,
-                                                       _ptr(dw)), "ungroup_grad")
-    return out if xs is None else (out, dw)
+    return _token_grad("mvr_ungroup_rows_grad_device", dout, plan.n, plan, weights, xs, "xs", plan.n_ids, plan.n_ids,
+                       out, ctx)
 
 
 __all__ = ["Plan", "plan", "lookup", "lookup_grad", "group", "group_grad", "ungroup", "ungroup_grad"]
