@@ -222,25 +222,33 @@ int spread(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t
   DeviceScope dev_scope(c);
   MVR_TRY(dev_scope.status);
   const uint64_t pairs = n * columns;
-  const int w_ = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {dw ? other : nullptr, os}});
-  return by_type(dtype, [&](auto* t) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    return by_vec<T>(w_, [&](auto vec) {
-      constexpr int V = decltype(vec)::value;
-      const uint32_t chunks = dim / V;
-      if (dw) {
-        const uint32_t L = lanes_of(c, pairs, chunks);
+  if (dw) {
+    const int width = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {other, os}});
+    return by_type(dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      return by_vec<T>(width, [&](auto vec) {
+        constexpr int V = decltype(vec)::value;
+        const uint32_t chunks = dim / V, L = lanes_of(c, pairs, chunks);
         spread_dot_kernel<T, V, true><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(
             L, chunks, (const T*)src, ss, columns, pairs, slot, w, (T*)dst, ds, (const T*)other, os, dw);
-      } else {
-        const Flat F = flat_of(n, chunks);
-        const bool several = many(c, F);
-        const auto kernel = several ? (columns <= 2 ? spread_kernel<T, V, 4, 2> : spread_kernel<T, V, 2, 8>)
-                                    : (columns <= 2 ? spread_kernel<T, V, 1, 2> : spread_kernel<T, V, 1, 8>);
-        const int per = several ? (columns <= 2 ? 1024 : 512) : 256;
-        kernel<<<blocks_of(F.total, per), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs, slot, w, (T*)dst,
-                                                               ds);
-      }
+        MVR_CUDA(c, cudaGetLastError());
+        return (int)MVR_OK;
+      });
+    });
+  }
+  const int width = vec_of(dtype, dim, {{src, ss}, {dst, ds}}, 32);
+  return by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return by_vec<T, 32>(width, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      constexpr int kMany = sizeof(T) * V == 32 ? 2 : 4;
+      const Flat F = flat_of(n, dim / V);
+      const bool several = F.total >= (uint64_t)kMany * 2048 * c->sm_count;
+      const auto kernel = several ? (columns <= 2 ? spread_kernel<T, V, kMany, 2> : spread_kernel<T, V, 2, 8>)
+                                  : (columns <= 2 ? spread_kernel<T, V, 1, 2> : spread_kernel<T, V, 1, 8>);
+      const int per = several ? (columns <= 2 ? 256 * kMany : 512) : 256;
+      kernel<<<blocks_of(F.total, per), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs, slot, w, (T*)dst,
+                                                             ds);
       MVR_CUDA(c, cudaGetLastError());
       return (int)MVR_OK;
     });

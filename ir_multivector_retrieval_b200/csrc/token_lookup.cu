@@ -13,9 +13,11 @@ namespace {
 // that a warp writes one run of memory whatever the row length; several of
 // them a thread, the block's stride apart, when there is work for all SMs. All
 // ids and scales are asked for before the first is used: the chain from an id
-// to its row is what a block's time consists of.
+// to its row is what a block's time consists of. 1,521,797 x 64 f32 from 32,768
+// rows with scales: 73 us (5.6 TB/s) with two accesses of 32 bytes a thread and
+// eight blocks an SM, 81 us with four of 16 bytes and six, 93 with eight.
 template <class T, class I, int V, int UR, bool SCALE>
-__global__ void __launch_bounds__(256, 6)
+__global__ void __launch_bounds__(256, sizeof(T) * V == 32 ? 8 : 6)
 lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, const I* __restrict__ ids,
               const float* __restrict__ scale, float alpha, T* __restrict__ out, uint64_t os) {
   const FlatBlock<UR> B(F);
@@ -53,7 +55,7 @@ lookup_kernel(Flat F, const T* __restrict__ table, uint32_t rows, uint64_t ts, c
 template <class T, class I, int V>
 int lookup_run(Ctx* c, uint64_t n, uint32_t chunks, const void* table, uint64_t rows, uint64_t ts, const void* ids,
                const float* scale, float alpha, void* out, uint64_t os) {
-  constexpr int kMany = 4;
+  constexpr int kMany = sizeof(T) * V == 32 ? 2 : 4;
   const Flat F = flat_of(n, chunks);
   const bool several = F.total >= (uint64_t)kMany * 2048 * c->sm_count;
   const auto kernel = scale ? (several ? lookup_kernel<T, I, V, kMany, true> : lookup_kernel<T, I, V, 1, true>)
@@ -587,10 +589,10 @@ int mvr_lookup_device(mvr_ctx* h, const void* d_table, int dtype, uint64_t rows,
   if (n == 0) return MVR_OK;
   mvr::DeviceScope dev_scope(c);
   MVR_TRY(dev_scope.status);
-  const int w = mvr::tok::vec_of(dtype, dim, {{d_table, table_stride}, {d_out, out_stride}});
+  const int w = mvr::tok::vec_of(dtype, dim, {{d_table, table_stride}, {d_out, out_stride}}, 32);
   return mvr::tok::by_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    return mvr::tok::by_vec<T>(w, [&](auto vec) {
+    return mvr::tok::by_vec<T, 32>(w, [&](auto vec) {
       constexpr int V = decltype(vec)::value;
       const auto run = id_bytes == 8 ? mvr::tok::lookup_run<T, uint64_t, V> : mvr::tok::lookup_run<T, uint32_t, V>;
       return run(c, n, dim / V, d_table, rows, table_stride, d_ids, d_scale, alpha, d_out, out_stride);
@@ -634,9 +636,8 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
     auto run = [&](auto* o) {
       using O = std::remove_pointer_t<decltype(o)>;
       int w = mvr::tok::vec_of(dtype, dim, {{d_grad, grad_stride}, {d_dscale ? d_table : nullptr, table_stride}});
-      // 8 f32 sums are two 16-byte accesses, so 16-byte alignment serves them too
-      const int wo = mvr::tok::vec_of(dtable_dtype, dim, {{d_dtable, dtable_stride}});
-      w = std::min(w, sizeof(O) > sizeof(T) && wo == 4 ? 8 : wo);
+      // beside 8 16-bit elements, 8 f32 sums are 32 bytes
+      w = std::min(w, mvr::tok::vec_of(dtable_dtype, dim, {{d_dtable, dtable_stride}}, 16 / sizeof(T) * sizeof(O)));
       return mvr::tok::by_vec<T>(w, [&](auto vec) {
         constexpr int V = decltype(vec)::value;
         mvr::tok::GradArgs<T, O, V> A;

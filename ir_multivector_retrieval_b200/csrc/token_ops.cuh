@@ -35,26 +35,27 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// V consecutive elements of a row as they lie in memory: 2 to 16 bytes (32
-// for f32 sums beside 8 16-bit elements), aligned to that size up to 16, so
-// each is one access or two. Rows in flight are kept in this form.
+// V consecutive elements of a row as they lie in memory: 2 to 32 bytes, aligned
+// to that size, so that each is one access. Rows in flight are kept in this
+// form.
 template <class T, int V>
 struct Raw {
   static constexpr int kBytes = (int)sizeof(T) * V;
   static constexpr int kWords = (kBytes + 3) / 4;
-  static_assert(kBytes <= 32, "one or two accesses");
+  static_assert(kBytes <= 32, "one access");
   uint32_t w[kWords];
 
   __device__ __forceinline__ void load(const T* __restrict__ p) {
-    if constexpr (kBytes >= 16) {
-#pragma unroll
-      for (int h = 0; h < kBytes / 16; ++h) {
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(p) + h);
-        w[h * 4] = r.x;
-        w[h * 4 + 1] = r.y;
-        w[h * 4 + 2] = r.z;
-        w[h * 4 + 3] = r.w;
-      }
+    if constexpr (kBytes == 32) {
+      asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(p));
+    } else if constexpr (kBytes == 16) {
+      const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = r.x;
+      w[1] = r.y;
+      w[2] = r.z;
+      w[3] = r.w;
     } else if constexpr (kBytes == 8) {
       const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
       w[0] = r.x;
@@ -66,30 +67,13 @@ struct Raw {
     }
   }
 
-  // the same from shared memory
-  __device__ __forceinline__ void read(const T* p) {
-    if constexpr (kBytes == 16) {
-      const uint4 r = *reinterpret_cast<const uint4*>(p);
-      w[0] = r.x;
-      w[1] = r.y;
-      w[2] = r.z;
-      w[3] = r.w;
-    } else if constexpr (kBytes == 8) {
-      const uint2 r = *reinterpret_cast<const uint2*>(p);
-      w[0] = r.x;
-      w[1] = r.y;
-    } else if constexpr (kBytes == 4) {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else {
-      w[0] = *reinterpret_cast<const unsigned short*>(p);
-    }
-  }
-
   __device__ __forceinline__ void store(T* p) const {
-    if constexpr (kBytes >= 16) {
-#pragma unroll
-      for (int h = 0; h < kBytes / 16; ++h)
-        reinterpret_cast<uint4*>(p)[h] = make_uint4(w[h * 4], w[h * 4 + 1], w[h * 4 + 2], w[h * 4 + 3]);
+    if constexpr (kBytes == 32) {
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                   "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    } else if constexpr (kBytes == 16) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     } else if constexpr (kBytes == 8) {
       *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     } else if constexpr (kBytes == 4) {
@@ -194,15 +178,15 @@ inline bool known(int dtype) { return dtype == MVR_F32 || dtype == MVR_BF16 || d
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline uint64_t up256(uint64_t v) { return (v + 255) & ~(uint64_t)255; }
 
-// Largest number of elements, at most 16 bytes, by which the row length, the
+// Largest number of elements, at most `most` bytes, by which the row length, the
 // strides and the addresses can all be divided: how wide a lane reads.
 struct Rows {
   const void* p;
   uint64_t stride;
 };
-inline int vec_of(int dtype, uint32_t dim, std::initializer_list<Rows> all) {
+inline int vec_of(int dtype, uint32_t dim, std::initializer_list<Rows> all, uint64_t most = 16) {
   const uint64_t e = elem_size(dtype);
-  uint64_t bits = 16 / e | dim;
+  uint64_t bits = most / e | dim;
   for (const Rows& r : all)
     if (r.p) bits |= r.stride | reinterpret_cast<uintptr_t>(r.p) / e;
   return (int)(bits & (~bits + 1));
@@ -221,9 +205,6 @@ inline Flat flat_of(uint64_t n, uint32_t chunks) {
   return {n * chunks, chunks, shift};
 }
 
-// Four elements a thread when that still fills every SM with threads.
-inline bool many(Ctx* c, const Flat& F) { return F.total >= 4ull * 2048 * c->sm_count; }
-
 // Lanes of a row for the dot products: as few as sixteen chunks a lane leave (the
 // exchanges between lanes cost more than the loop), while every SM keeps 1024
 // threads.
@@ -238,12 +219,13 @@ inline unsigned blocks_of(uint64_t items, uint64_t per_block) {
   return (unsigned)((items + per_block - 1) / per_block);
 }
 
-// Calls f with the width as a compile-time number.
-template <class T, class F>
+// Calls f with the width as a compile-time number, at most MOST bytes.
+template <class T, int MOST = 16, class F>
 int by_vec(int v, F&& f) {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (MOST / sizeof(T) >= 16)
+    if (v >= 16) return f(std::integral_constant<int, 16>());
+  if constexpr (MOST / sizeof(T) >= 8)
     if (v >= 8) return f(std::integral_constant<int, 8>());
-  }
   if (v >= 4) return f(std::integral_constant<int, 4>());
   if (v >= 2) return f(std::integral_constant<int, 2>());
   return f(std::integral_constant<int, 1>());
