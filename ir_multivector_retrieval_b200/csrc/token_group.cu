@@ -100,62 +100,92 @@ collect_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns,
 }
 
 // The pair's two rows in one pass: dst[slot] = w * src[token], dw = <src[token],
-// other[slot]>. A group of lanes has a pair, so a token's row is read once
-// from memory and again from the caches for its other choices.
-template <class T, int V, bool DST>
+// other[slot]>. A group of L lanes has a pair, so a token's row is read once
+// from memory and again from the caches for its other choices. Rows that L
+// lanes hold at once are taken PU at a time, longer ones CU chunks at a time.
+template <class T, int V, int PU, int CU, bool DST>
 __global__ void __launch_bounds__(256)
 spread_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint64_t ss, uint32_t columns,
                   uint64_t pairs, const uint32_t* __restrict__ slot, const float* __restrict__ w,
                   T* __restrict__ dst, uint64_t ds, const T* __restrict__ other, uint64_t other_s,
                   float* __restrict__ dw) {
-  constexpr int U = 4;
   __shared__ float s_sum[8];
-  const uint32_t l = threadIdx.x & (L - 1);
-  const uint64_t pair = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const uint32_t p = pair < pairs ? slot[pair] : kNoSlot;
-  float dot = 0.f;
-  if (p < pairs) {
-    const T* a = src + pair / columns * ss;
-    const T* b = other + p * other_s;
-    const float f = w ? w[pair] : 1.f;
-    for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
-      Raw<T, V> x[U], o[U];
+  const uint32_t l = threadIdx.x & (L - 1), G = 256 / L;
+  const uint64_t first = (uint64_t)blockIdx.x * (G * PU) + threadIdx.x / L;
+  uint32_t p[PU];
+  float f[PU], dot[PU];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        x[u].zero();
-        o[u].zero();
+  for (int q = 0; q < PU; ++q) {
+    const uint64_t pair = first + q * G;
+    p[q] = pair < pairs ? slot[pair] : kNoSlot;
+    dot[q] = 0.f;
+  }
+#pragma unroll
+  for (int q = 0; q < PU; ++q) f[q] = w && p[q] < pairs ? w[first + q * G] : 1.f;
+  for (uint32_t c0 = l; c0 < chunks; c0 += CU * L) {
+    Raw<T, V> x[PU][CU], o[PU][CU];
+#pragma unroll
+    for (int q = 0; q < PU; ++q)
+#pragma unroll
+      for (int u = 0; u < CU; ++u) {
+        x[q][u].zero();
+        o[q][u].zero();
         const uint32_t c = c0 + u * L;
-        if (c < chunks) {
-          x[u].load(a + (uint64_t)c * V);
-          o[u].load(b + (uint64_t)c * V);
+        if (p[q] < pairs && c < chunks) {
+          x[q][u].load(src + (first + q * G) / columns * ss + (uint64_t)c * V);
+          o[q][u].load(other + p[q] * other_s + (uint64_t)c * V);
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+    for (int q = 0; q < PU; ++q)
+#pragma unroll
+      for (int u = 0; u < CU; ++u) {
         float y[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          dot = fmaf(x[u].get(v), o[u].get(v), dot);
-          y[v] = f * x[u].get(v);
+          dot[q] = fmaf(x[q][u].get(v), o[q][u].get(v), dot[q]);
+          y[v] = f[q] * x[q][u].get(v);
         }
         if constexpr (DST) {
           const uint32_t c = c0 + u * L;
-          if (c < chunks) {
-            if (w) x[u].set(y);
-            x[u].store(dst + p * ds + (uint64_t)c * V);
+          if (p[q] < pairs && c < chunks) {
+            if (w) x[q][u].set(y);
+            x[q][u].store(dst + p[q] * ds + (uint64_t)c * V);
           }
         }
       }
-    }
   }
-  dot = group_sum(dot, L, s_sum);
-  if (l == 0 && pair < pairs) dw[pair] = dot;
+  if constexpr (PU == 1) {
+    dot[0] = group_sum(dot[0], L, s_sum);
+    if (l == 0 && first < pairs) dw[first] = dot[0];
+  } else {  // L is at most a warp here
+    const GroupSums<PU> sums(dot, L, l);
+    if (sums.writes)
+#pragma unroll 1
+      for (int k = 0; k < sums.values; ++k) {
+        const uint64_t pair = first + (sums.which + k) * G;
+        if (pair < pairs) dw[pair] = sums.at(dot, k);
+      }
+  }
+}
+
+template <class T, int V, bool DST>
+int spread_dot(Ctx* c, uint32_t chunks, const T* src, uint64_t ss, uint32_t columns, uint64_t pairs,
+               const uint32_t* slot, const float* w, T* dst, uint64_t ds, const T* other, uint64_t os, float* dw) {
+  constexpr int U = sizeof(T) * V == 32 ? 2 : 4;
+  const uint32_t L = lanes_of(c, pairs, chunks);
+  const bool narrow = chunks <= L && L <= 32;
+  const auto kernel = narrow ? spread_dot_kernel<T, V, U, 1, DST> : spread_dot_kernel<T, V, 1, U, DST>;
+  kernel<<<blocks_of(pairs, narrow ? 256 / L * U : 256 / L), 256, 0, c->stream>>>(L, chunks, src, ss, columns, pairs,
+                                                                                 slot, w, dst, ds, other, os, dw);
+  MVR_CUDA(c, cudaGetLastError());
+  return MVR_OK;
 }
 
 // dst[i] = sum_c w * src[slot] and dw = <other[i], src[slot]> in one pass, for
 // at most KU choices: a group of lanes has a token.
 template <class T, int V, int KU>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 collect_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint64_t ss, uint64_t n, uint32_t columns,
                    const uint32_t* __restrict__ slot, const float* __restrict__ w, T* __restrict__ dst, uint64_t ds,
                    const T* __restrict__ other, uint64_t other_s, float* __restrict__ dw) {
@@ -172,7 +202,7 @@ collect_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint6
     f[k] = p[k] < pairs ? (w ? w[i * columns + k] : 1.f) : 0.f;
     dot[k] = 0.f;
   }
-  constexpr int U = KU <= 4 ? 2 : 1;  // chunks at once: eight rows' in flight
+  constexpr int U = KU <= 4 && sizeof(T) * V < 32 ? 2 : 1;  // chunks at once
   if (i < n)
     for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
       Raw<T, V> o[U], x[U][KU];
@@ -223,16 +253,13 @@ int spread(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_t
   MVR_TRY(dev_scope.status);
   const uint64_t pairs = n * columns;
   if (dw) {
-    const int width = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {other, os}});
+    const int width = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {other, os}}, 32);
     return by_type(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      return by_vec<T>(width, [&](auto vec) {
+      return by_vec<T, 32>(width, [&](auto vec) {
         constexpr int V = decltype(vec)::value;
-        const uint32_t chunks = dim / V, L = lanes_of(c, pairs, chunks);
-        spread_dot_kernel<T, V, true><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(
-            L, chunks, (const T*)src, ss, columns, pairs, slot, w, (T*)dst, ds, (const T*)other, os, dw);
-        MVR_CUDA(c, cudaGetLastError());
-        return (int)MVR_OK;
+        return spread_dot<T, V, true>(c, dim / V, (const T*)src, ss, columns, pairs, slot, w, (T*)dst, ds,
+                                      (const T*)other, os, dw);
       });
     });
   }
@@ -264,32 +291,53 @@ int collect(Ctx* c, const void* src, int dtype, uint64_t ss, uint64_t n, uint32_
   DeviceScope dev_scope(c);
   MVR_TRY(dev_scope.status);
   const uint64_t pairs = n * columns;
-  const int w_ = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {dw ? other : nullptr, os}});
-  return by_type(dtype, [&](auto* t) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    return by_vec<T>(w_, [&](auto vec) {
-      constexpr int V = decltype(vec)::value;
-      const uint32_t chunks = dim / V;
-      const T *s = (const T*)src, *o = (const T*)other;
-      if (dw && columns <= kDotColumns) {
+  if (dw && columns <= kDotColumns) {
+    // one or two rows beside the token's own: 32 bytes of each a lane (251 us, with 16 396 us, at 1,521,797 x 2 x
+    // 64 f32); more of them are enough in flight with 16 (66 us, with 32 77 us, at 8192 x 8 x 2048 bf16)
+    const int most = columns <= 2 ? 32 : 16;
+    const int width = vec_of(dtype, dim, {{src, ss}, {dst, ds}, {other, os}}, most);
+    return by_type(dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      auto launch = [&](auto kernel, uint32_t chunks) {
         const uint32_t L = lanes_of(c, n, chunks);
-        const unsigned blocks = blocks_of(n, 256 / L);
-        const auto kernel = columns <= 2   ? collect_dot_kernel<T, V, 2>
-                            : columns <= 4 ? collect_dot_kernel<T, V, 4>
-                                           : collect_dot_kernel<T, V, kDotColumns>;
-        kernel<<<blocks, 256, 0, c->stream>>>(L, chunks, s, ss, n, columns, slot, w, (T*)dst, ds, o, os, dw);
-      } else {
-        const Flat F = flat_of(n, chunks);
-        const auto kernel = columns <= 2 ? collect_kernel<T, V, 2> : collect_kernel<T, V, 4>;
-        kernel<<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, s, ss, columns, pairs, slot, w, (T*)dst, ds);
-        if (dw) {  // the dots on their own: src once more
-          const uint32_t L = lanes_of(c, pairs, chunks);
-          spread_dot_kernel<T, V, false><<<blocks_of(pairs, 256 / L), 256, 0, c->stream>>>(
-              L, chunks, o, os, columns, pairs, slot, nullptr, nullptr, 0, s, ss, dw);
-        }
-      }
+        kernel<<<blocks_of(n, 256 / L), 256, 0, c->stream>>>(L, chunks, (const T*)src, ss, n, columns, slot, w, (T*)dst,
+                                                             ds, (const T*)other, os, dw);
+        MVR_CUDA(c, cudaGetLastError());
+        return (int)MVR_OK;
+      };
+      if (columns <= 2)
+        return by_vec<T, 32>(width, [&](auto vec) {
+          constexpr int V = decltype(vec)::value;
+          return launch(collect_dot_kernel<T, V, 2>, dim / V);
+        });
+      return by_vec<T>(width, [&](auto vec) {
+        constexpr int V = decltype(vec)::value;
+        return launch(columns <= 4 ? collect_dot_kernel<T, V, 4> : collect_dot_kernel<T, V, kDotColumns>, dim / V);
+      });
+    });
+  }
+  const int width = vec_of(dtype, dim, {{src, ss}, {dst, ds}}, 32);
+  MVR_TRY(by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return by_vec<T, 32>(width, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      const Flat F = flat_of(n, dim / V);
+      const auto kernel = columns <= 2 ? collect_kernel<T, V, 2> : collect_kernel<T, V, 4>;
+      kernel<<<blocks_of(F.total, 256), 256, 0, c->stream>>>(F, (const T*)src, ss, columns, pairs, slot, w, (T*)dst,
+                                                             ds);
       MVR_CUDA(c, cudaGetLastError());
       return (int)MVR_OK;
+    });
+  }));
+  if (!dw) return MVR_OK;
+  // more choices than a lane holds dot products of: those on their own, src once more
+  const int dot_width = vec_of(dtype, dim, {{src, ss}, {other, os}}, 32);
+  return by_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return by_vec<T, 32>(dot_width, [&](auto vec) {
+      constexpr int V = decltype(vec)::value;
+      return spread_dot<T, V, false>(c, dim / V, (const T*)other, os, columns, pairs, slot, nullptr, nullptr, 0,
+                                     (const T*)src, ss, dw);
     });
   });
 }

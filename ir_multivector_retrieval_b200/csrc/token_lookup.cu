@@ -139,41 +139,6 @@ __device__ __forceinline__ void fill_empty_rows(const GradShape& S, const uint32
       for (uint32_t c = lane & (L - 1); c < chunks; c += L) z.store(dtable + (v0 + j) * S.ds + (uint64_t)c * V);
 }
 
-// Sums of U values over the L lanes of a group, all at once: while a lane has
-// several values, it gives half of them to the lane across and takes the other
-// half's, so they take U - 1 + log2(L / U) exchanges instead of U log2(L).
-template <int U>
-struct GroupSums {
-  uint32_t which = 0;  // x[k] has become the sum of value which + k, k < values
-  int values = U;      // one unless the group has fewer lanes than U
-  bool writes;         // whether this lane is the one to write them
-  __device__ __forceinline__ GroupSums(float (&x)[U], uint32_t L, uint32_t l) {
-    uint32_t o = L >> 1;
-#pragma unroll
-    for (int half = U >> 1; half > 0; half >>= 1) {
-      if (o == 0) continue;  // the same for all lanes
-      const bool up = l & o;
-#pragma unroll
-      for (int k = 0; k < half; ++k) {
-        const float give = up ? x[k] : x[k + half];
-        const float keep = up ? x[k + half] : x[k];
-        x[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-      }
-      which += up ? half : 0;
-      values = half;
-      o >>= 1;
-    }
-    writes = o == 0 || (l & (2 * o - 1)) == 0;
-    for (; o > 0; o >>= 1) x[0] += __shfl_xor_sync(0xffffffffu, x[0], o);
-  }
-  static __device__ __forceinline__ float at(const float (&x)[U], int k) {
-    float r = x[0];
-#pragma unroll
-    for (int q = 1; q < U; ++q) r = k == q ? x[q] : r;
-    return r;
-  }
-};
-
 // Places of a tile whose plan entries a block keeps in shared memory.
 constexpr uint32_t kMaxTile = 2048;
 constexpr int kFlight = 4;  // rows a lane takes at once

@@ -145,6 +145,41 @@ __device__ __forceinline__ float group_sum(float x, uint32_t L, float* s) {
   return x;
 }
 
+// Sums of U values over the L lanes of a group, all at once: while a lane has
+// several values, it gives half of them to the lane across and takes the other
+// half's, so they take U - 1 + log2(L / U) exchanges instead of U log2(L).
+template <int U>
+struct GroupSums {
+  uint32_t which = 0;  // x[k] has become the sum of value which + k, k < values
+  int values = U;      // one unless the group has fewer lanes than U
+  bool writes;         // whether this lane is the one to write them
+  __device__ __forceinline__ GroupSums(float (&x)[U], uint32_t L, uint32_t l) {
+    uint32_t o = L >> 1;
+#pragma unroll
+    for (int half = U >> 1; half > 0; half >>= 1) {
+      if (o == 0) continue;  // the same for all lanes
+      const bool up = l & o;
+#pragma unroll
+      for (int k = 0; k < half; ++k) {
+        const float give = up ? x[k] : x[k + half];
+        const float keep = up ? x[k + half] : x[k];
+        x[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+      which += up ? half : 0;
+      values = half;
+      o >>= 1;
+    }
+    writes = o == 0 || (l & (2 * o - 1)) == 0;
+    for (; o > 0; o >>= 1) x[0] += __shfl_xor_sync(0xffffffffu, x[0], o);
+  }
+  static __device__ __forceinline__ float at(const float (&x)[U], int k) {
+    float r = x[0];
+#pragma unroll
+    for (int q = 1; q < U; ++q) r = k == q ? x[q] : r;
+    return r;
+  }
+};
+
 // Where element `e` of the outputs lies: row and chunk of a row. `shift` is
 // log2(chunks) or -1.
 struct Flat {
@@ -205,12 +240,12 @@ inline Flat flat_of(uint64_t n, uint32_t chunks) {
   return {n * chunks, chunks, shift};
 }
 
-// Lanes of a row for the dot products: as few as sixteen chunks a lane leave (the
-// exchanges between lanes cost more than the loop), while every SM keeps 1024
-// threads.
+// Lanes of a row for the dot products: a warp where the row fills one (fewer
+// would read pieces of lines, more have to meet in shared memory), several
+// while that leaves an SM short of 1024 threads.
 inline uint32_t lanes_of(Ctx* c, uint64_t n, uint32_t chunks) {
   uint32_t L = std::min(256u, pow2_ceil(chunks));
-  while (L > 1 && chunks < 16 * L && n * (L / 2) >= 1024ull * c->sm_count) L /= 2;
+  while (L > 32 && n * (L / 2) >= 1024ull * c->sm_count) L /= 2;
   return L;
 }
 
