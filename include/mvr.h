@@ -740,10 +740,9 @@ int mvr_lookup_grad_bytes(uint64_t n_ids, uint32_t dim, uint64_t* bytes);
  * and may be NULL otherwise. */
 int mvr_lookup_grad_device(mvr_ctx* ctx, const void* d_grad, int dtype, uint64_t grad_stride, uint64_t n_ids,
                            uint64_t rows, uint32_t dim, const uint32_t* d_offsets, const uint32_t* d_order,
-                           const uint32_t* d_keys, const uint32_t* d_slot, const float* d_scale, float alpha,
-                           const void* d_table, uint64_t table_stride, void* d_dtable, int dtable_dtype,
-                           uint64_t dtable_stride, int accumulate, float* d_dscale, void* d_workspace,
-                           uint64_t workspace_bytes);
+                           const uint32_t* d_keys, const float* d_scale, float alpha, const void* d_table,
+                           uint64_t table_stride, void* d_dtable, int dtable_dtype, uint64_t dtable_stride,
+                           int accumulate, float* d_dscale, void* d_workspace, uint64_t workspace_bytes);
 
 /* Rows into sorted order. Each of n tokens has `columns` ids; slot is that of
  * the plan of the n x columns ids, weights n x columns (NULL: ones):

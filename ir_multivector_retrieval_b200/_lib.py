@@ -258,7 +258,7 @@ SIGNATURES = {
     "mvr_token_plan_device": (C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, _P, _P, _P, _P, _P, C.c_uint64]),
     "mvr_lookup_grad_bytes": (C.c_int, [C.c_uint64, C.c_uint32, _U64]),
     "mvr_lookup_grad_device": (
-        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, _P, _P, _P, _P, _P, C.c_float, _P,
+        C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, _P, _P, _P, _P, C.c_float, _P,
                   C.c_uint64, _P, C.c_int, C.c_uint64, C.c_int, _P, _P, C.c_uint64]),
     "mvr_group_rows_device": (
         C.c_int, [_P, _P, C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_uint64]),

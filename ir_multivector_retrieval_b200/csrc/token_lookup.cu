@@ -91,6 +91,7 @@ struct GradShape {
   uint32_t per_group;  // Tg: places of a group
   uint32_t fills;      // blocks that fill rows without a token, before those with places
   uint32_t tiles;
+  uint32_t dots;       // blocks behind them for dscale, where a row's parts lie in several blocks
   uint32_t fill_lanes;  // lanes of a row there, a power of two
   uint64_t gs, ts, ds;  // row strides of grad, table, dtable
 };
@@ -139,6 +140,45 @@ __device__ __forceinline__ void fill_empty_rows(const GradShape& S, const uint32
       for (uint32_t c = lane & (L - 1); c < chunks; c += L) z.store(dtable + (v0 + j) * S.ds + (uint64_t)c * V);
 }
 
+// dscale of rows whose parts lie in several blocks: a warp per place, beside
+// the blocks that sum, whose time is mostly waiting.
+template <class T, class O, int V>
+__device__ __forceinline__ void scale_dots(const GradArgs<T, O, V>& A) {
+  constexpr int U = 4;
+  const GradShape& S = A.s;
+  const uint64_t block = (uint64_t)(blockIdx.x - S.fills - S.tiles) * gridDim.y + blockIdx.y;
+  const uint64_t p = block * 8 + (threadIdx.x >> 5);
+  if (p >= S.n) return;
+  const uint32_t lane = threadIdx.x & 31, chunks = S.dim / V;
+  const uint32_t i = A.order[p], r = A.keys[p];
+  if (i >= S.n) return;
+  float dot = 0.f;
+  if (r < S.rows) {
+    const T* a = A.grad + i * S.gs;
+    const T* b = A.table + r * S.ts;
+    for (uint32_t c0 = lane; c0 < chunks; c0 += U * 32) {
+      Raw<T, V> x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u].zero();
+        y[u].zero();
+        const uint32_t c = c0 + u * 32;
+        if (c < chunks) {
+          x[u].load(a + (uint64_t)c * V);
+          y[u].load(b + (uint64_t)c * V);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) dot = fmaf(x[u].get(v), y[u].get(v), dot);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+  if (lane == 0) A.dscale[i] = A.alpha * dot;
+}
+
 // Places of a tile whose plan entries a block keeps in shared memory.
 constexpr uint32_t kMaxTile = 2048;
 constexpr int kFlight = 4;  // rows a lane takes at once
@@ -159,6 +199,12 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   if (blockIdx.x < S.fills) {
     fill_empty_rows<O, V>(S, A.offsets, A.dtable);
     return;
+  }
+  if constexpr (!DSCALE) {
+    if (blockIdx.x >= S.fills + S.tiles) {
+      scale_dots(A);
+      return;
+    }
   }
   const uint32_t tile_at = blockIdx.x - S.fills;
   const uint32_t L = S.lanes, G = 256 / L;
@@ -448,50 +494,12 @@ lookup_grad_join_kernel(GradShape S, uint32_t L, uint32_t tile, const uint32_t* 
   }
 }
 
-// dscale where a row's parts lie in several blocks of the sums: a group of L
-// lanes per token, its table row is the key at its place.
-template <class T, int V>
-__global__ void __launch_bounds__(256)
-lookup_dscale_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ grad, uint64_t gs, uint32_t n, uint32_t rows,
-                     const uint32_t* __restrict__ keys, const uint32_t* __restrict__ slot, float alpha,
-                     const T* __restrict__ table, uint64_t ts, float* __restrict__ dscale) {
-  constexpr int U = 4;
-  __shared__ float s_sum[8];
-  const uint32_t l = threadIdx.x & (L - 1);
-  const uint64_t i = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const uint32_t p = i < n ? slot[i] : kNoSlot, r = p < n ? keys[p] : rows;
-  float dot = 0.f;
-  if (r < rows) {
-    const T* a = grad + i * gs;
-    const T* b = table + r * ts;
-    for (uint32_t c0 = l; c0 < chunks; c0 += U * L) {
-      Raw<T, V> x[U], o[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        x[u].zero();
-        o[u].zero();
-        const uint32_t c = c0 + u * L;
-        if (c < chunks) {
-          x[u].load(a + (uint64_t)c * V);
-          o[u].load(b + (uint64_t)c * V);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int v = 0; v < V; ++v) dot = fmaf(x[u].get(v), o[u].get(v), dot);
-    }
-  }
-  dot = group_sum(dot, L, s_sum);
-  if (l == 0 && i < n) dscale[i] = alpha * dot;
-}
-
 // Smallest block of places, whatever the row length: the workspace is sized
 // for it. 8 places a group, 8 groups of 32 lanes at least.
 constexpr uint32_t kMinTile = 64;
 
 template <class T, class O, int V>
-int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
+int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A) {
   GradShape& S = A.s;
   cudaStream_t st = c->stream;
   constexpr uint32_t NCH = chunks_per_lane<T, V>();
@@ -511,12 +519,12 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
   S.tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
   S.fill_lanes = std::min(32u, pow2_ceil(chunks));
   S.fills = A.accumulate ? 0 : (uint32_t)(((S.rows + kFillRows - 1ull) / kFillRows + slabs - 1) / slabs);
-  if (S.tiles + S.fills == 0) return MVR_OK;
   const bool with_dscale = A.dscale && slabs == 1;
+  S.dots = A.dscale && !with_dscale ? (uint32_t)(((S.n + 7ull) / 8 + slabs - 1) / slabs) : 0;
+  if (S.tiles + S.fills == 0) return MVR_OK;
   const auto kernel = with_dscale ? lookup_grad_tile_kernel<T, O, V, true> : lookup_grad_tile_kernel<T, O, V, false>;
-  const size_t smem = grad_smem(tile);
-  MVR_CUDA(c, raise_smem_limit((const void*)kernel, smem));
-  MVR_CUDA(c, launch_pdl(kernel, dim3(S.fills + S.tiles, slabs), 256, smem, st, A));
+  const size_t smem = grad_smem(tile);  // with the kernel's own below the 48 KB that need no request
+  MVR_CUDA(c, launch_pdl(kernel, dim3(S.fills + S.tiles + S.dots, slabs), 256, smem, st, A));
   if (S.tiles > 1) {  // a block's columns once, while the grid stays small: most blocks have nothing to join
     const uint32_t w = S.dim % 4 == 0 ? 4 : 1, L = std::min(32u, pow2_ceil(S.dim / w));
     const uint32_t columns = (S.dim + L * w - 1) / (L * w);
@@ -524,12 +532,6 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A, const uint32_t* slot) {
     const auto join = w == 4 ? lookup_grad_join_kernel<O, 4> : lookup_grad_join_kernel<O, 1>;
     MVR_CUDA(c, launch_pdl(join, grid, kJoinThreads, 0, st, S, L, tile, A.offsets, A.keys, A.part, A.dtable, A.alpha,
                            A.accumulate));
-  }
-  if (A.dscale && S.tiles && !with_dscale) {  // a row's parts lie in several blocks
-    const uint32_t L = lanes_of(c, S.n, chunks);
-    lookup_dscale_kernel<T, V><<<blocks_of(S.n, 256 / L), 256, 0, st>>>(L, chunks, A.grad, S.gs, S.n, S.rows, A.keys,
-                                                                       slot, A.alpha, A.table, S.ts, A.dscale);
-    MVR_CUDA(c, cudaGetLastError());
   }
   return MVR_OK;
 }
@@ -573,10 +575,9 @@ int mvr_lookup_grad_bytes(uint64_t n_ids, uint32_t dim, uint64_t* bytes) {
 
 int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t grad_stride, uint64_t n_ids,
                            uint64_t rows, uint32_t dim, const uint32_t* d_offsets, const uint32_t* d_order,
-                           const uint32_t* d_keys, const uint32_t* d_slot, const float* d_scale, float alpha,
-                           const void* d_table, uint64_t table_stride, void* d_dtable, int dtable_dtype,
-                           uint64_t dtable_stride, int accumulate, float* d_dscale, void* d_workspace,
-                           uint64_t workspace_bytes) {
+                           const uint32_t* d_keys, const float* d_scale, float alpha, const void* d_table,
+                           uint64_t table_stride, void* d_dtable, int dtable_dtype, uint64_t dtable_stride,
+                           int accumulate, float* d_dscale, void* d_workspace, uint64_t workspace_bytes) {
   if (!h) return MVR_E_INVALID_ARGUMENT;
   Ctx* c = &h->impl;
   MVR_TRY(mvr::tok::check_rows(c, "grad", d_grad, dtype, n_ids, dim, grad_stride, false));
@@ -584,8 +585,8 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
   if (n_ids > mvr::tok::kMaxIds) return mvr::tok::bad(c, "more than 2^31 - 1 ids");
   if (dtable_dtype != dtype && dtable_dtype != MVR_F32) return mvr::tok::bad(c, "dtable must have grad's type or f32");
   MVR_TRY(mvr::tok::check_rows(c, "dtable", d_dtable, dtable_dtype, rows, dim, dtable_stride, true));
-  if (!d_offsets || (n_ids && (!d_order || !d_keys || !d_slot))) return mvr::tok::bad(c, "null pointer: plan");
-  if (!mvr::tok::aligned(d_offsets, 4) || !mvr::tok::aligned(d_order, 4) || !mvr::tok::aligned(d_keys, 4) || !mvr::tok::aligned(d_slot, 4))
+  if (!d_offsets || (n_ids && (!d_order || !d_keys))) return mvr::tok::bad(c, "null pointer: plan");
+  if (!mvr::tok::aligned(d_offsets, 4) || !mvr::tok::aligned(d_order, 4) || !mvr::tok::aligned(d_keys, 4))
     return mvr::tok::bad(c, "the plan is not aligned to its type");
   MVR_TRY(mvr::tok::check_f32(c, "scale", d_scale));
   MVR_TRY(mvr::tok::check_f32(c, "dscale", d_dscale));
@@ -606,7 +607,7 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
       return mvr::tok::by_vec<T>(w, [&](auto vec) {
         constexpr int V = decltype(vec)::value;
         mvr::tok::GradArgs<T, O, V> A;
-        A.s = {n, v, dim, 0, 0, 0, 0, 0, grad_stride, table_stride, dtable_stride};
+        A.s = {n, v, dim, 0, 0, 0, 0, 0, 0, grad_stride, table_stride, dtable_stride};
         A.grad = (const T*)d_grad;
         A.offsets = d_offsets;
         A.order = d_order;
@@ -618,7 +619,7 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
         A.accumulate = accumulate;
         A.dscale = d_dscale;
         A.part = (float*)d_workspace;
-        return mvr::tok::lookup_grad_run(c, A, d_slot);
+        return mvr::tok::lookup_grad_run(c, A);
       });
     };
     if (dtable_dtype == MVR_F32) return run(static_cast<float*>(nullptr));

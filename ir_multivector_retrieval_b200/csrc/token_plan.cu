@@ -379,6 +379,11 @@ __global__ void __launch_bounds__(256) plan_borders_kernel(PlanArgs A) {
       s_place[g] = p;
       gap = 0;
     }
+    if (gap == 1) {  // the most when there are few rows
+      A.offsets[lo[q]] = p;
+      gap = 0;
+    }
+    if (!__any_sync(0xffffffffu, gap != 0)) continue;
     uint32_t end = gap;  // of the gaps up to this lane's
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -458,8 +463,7 @@ int plan_small(Ctx* c, const PlanArgs& A, const Digits& D, uint32_t* k0, uint32_
   const uint32_t blocks = std::min(kSmallBlocks, pow2_ceil((A.n + 256u - 1) / 256u));
   const uint32_t chunk = (A.n + blocks - 1) / blocks;
   const uint32_t rounds = (chunk + threads - 1) / threads;
-  const size_t smem = (3 + (size_t)threads / 32) * R * 4;
-  MVR_CUDA(c, raise_smem_limit((const void*)plan_small_kernel<I>, smem));
+  const size_t smem = (3 + (size_t)threads / 32) * R * 4;  // 44 KB at most: needs no request
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = blocks;
   cfg.blockDim = threads;
@@ -482,12 +486,11 @@ int plan_pass_of(Ctx* c, const PlanArgs& A, const void* kin, const uint32_t* vin
   cudaStream_t st = c->stream;
   constexpr uint32_t kTile = kTileThreads * ROUNDS;
   const uint32_t tiles = (uint32_t)((A.n + (kTile - 1ull)) / kTile), R = 1u << bits;
-  const size_t smem = (2 * R + std::max(kTileThreads / 32 * R, 2 * kTile)) * 4;
+  const size_t smem = (2 * R + std::max(kTileThreads / 32 * R, 2 * kTile)) * 4;  // 40 KB at most: needs no request
   const auto count = plan_hist_kernel<I, ROUNDS>;
   MVR_CUDA(c, launch_pdl(count, tiles, kTileThreads, 0, st, kin, A.n, A.rows, shift, R, tiles, hist));
   MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
   const auto scatter = last ? plan_scatter_kernel<I, ROUNDS, true> : plan_scatter_kernel<I, ROUNDS, false>;
-  MVR_CUDA(c, raise_smem_limit((const void*)scatter, smem));
   MVR_CUDA(c, launch_pdl(scatter, tiles, kTileThreads, smem, st, A, kin, vin, shift, bits, tiles, hist, sums, kout,
                          vout));
   return MVR_OK;
@@ -535,7 +538,8 @@ int mvr_token_plan_device(mvr_ctx* h, const void* d_ids, int id_bytes, uint64_t 
   MVR_TRY(mvr::tok::check_ids(c, d_ids, id_bytes, n_ids, rows));
   if (n_ids > mvr::tok::kMaxIds) return mvr::tok::bad(c, "more than 2^31 - 1 ids");
   if (!d_offsets || (n_ids && (!d_order || !d_keys || !d_slot))) return mvr::tok::bad(c, "null pointer");
-  if (!mvr::tok::aligned(d_offsets, 4) || !mvr::tok::aligned(d_order, 4) || !mvr::tok::aligned(d_keys, 4) || !mvr::tok::aligned(d_slot, 4))
+  if (!mvr::tok::aligned(d_offsets, 4) || !mvr::tok::aligned(d_order, 4) || !mvr::tok::aligned(d_keys, 4) ||
+      !mvr::tok::aligned(d_slot, 4))
     return mvr::tok::bad(c, "an output is not aligned to its type");
   uint64_t need = 0;
   MVR_TRY(mvr_token_plan_bytes(n_ids, rows, &need));

@@ -296,10 +296,9 @@ def plan(ids, rows: int, *, ctx=None) -> Plan:
     with scope:
         ids = ids.contiguous()
         i32 = _types()["i32"]
-        offsets = ids.new_empty(rows + 1, dtype=i32)
-        order = ids.new_empty(n, dtype=i32)
-        keys = ids.new_empty(n, dtype=i32)
-        slot = ids.new_empty(ids.shape, dtype=i32)
+        offsets, order, keys, slot = ids.new_empty(rows + 1 + 3 * n, dtype=i32).split((rows + 1, n, n, n))
+        if ids.dim() == 2:
+            slot = slot.view(ids.shape)
         need = _plan_bytes(n, rows)
         ws = _workspace(ids, need)
         _run(ctx, device, lambda lib, h: lib.mvr_token_plan_device(
@@ -372,7 +371,7 @@ def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None,
         ws = _workspace(g, need)
         _run(ctx, device, lambda lib, h: lib.mvr_lookup_grad_device(
             h, g.data_ptr(), dt, gs, n, rows, dim, plan.offsets.data_ptr(), plan.order.data_ptr(),
-            plan.keys.data_ptr(), plan.slot.data_ptr(), _ptr(scale), alpha, tp, ts, po, odt, so, int(accumulate),
+            plan.keys.data_ptr(), _ptr(scale), alpha, tp, ts, po, odt, so, int(accumulate),
             _ptr(dscale), _ptr(ws), need))
     return out if dscale is None else (out, dscale)
 
