@@ -429,8 +429,9 @@ struct Digits {
 // launches at some 10,000 pairs.
 bool is_small(uint64_t n, const Digits& D) { return n <= (D.passes == 1 ? kSmallMax : kSmallMaxPasses); }
 
-// Pairs a thread of a tile: few until the blocks are more than share the SMs.
-constexpr uint32_t kFewRounds = 4, kManyRounds = 8;
+// Pairs a thread of a tile: few until the blocks are more than share the SMs
+// (then the most that 64 registers hold: 47 us at 1,521,797 pairs, with 8 50).
+constexpr uint32_t kFewRounds = 4, kManyRounds = 11;
 bool few_rounds(uint64_t n) { return n <= 148ull * 4 * kFewRounds * kTileThreads; }
 
 // Workspace: two sets of pairs for the passes, and the counts of the tiles.

@@ -215,6 +215,21 @@ def test_lookup_grad(dtype, n, rows, dim, spread, scaled):
     assert bool((dt[empty] == 0).all())
 
 
+@pytest.mark.parametrize("n,rows,dim", [(70_000, 40, 128), (300_000, 5000, 64), (262_145, 100_000, 32), (9000, 70_000, 512)])
+def test_lookup_grad_of_many_tokens_with_64_bit_ids(n, rows, dim):
+    g = gen(n)
+    ids = make_ids(g, (n,), rows, torch.int64, "head", pad=0.02)
+    p = tokens.plan(ids, rows)
+    offsets, order, keys, slot, valid = plan_of(ids, rows)
+    assert torch.equal(p.offsets.long(), offsets) and torch.equal(p.slot.long(), slot)
+    assert torch.equal(p.order.long(), order) and torch.equal(p.keys.long(), keys)  # those that name no row last
+    grad, table = normal(g, n, dim, dtype=BF16), normal(g, rows, dim, dtype=BF16)
+    dt, ds = tokens.lookup_grad(grad, p, alpha=0.5, table=table, out=torch.empty(rows, dim, device="cuda"))
+    lookup_grad_check(grad, ids, rows, None, 0.5, dt)
+    prod = 0.5 * grad.double() * lookup_ref(table, ids, None, 1.0)
+    within(ds, prod.sum(1), 1.001 * (dim + 2) * U32 * prod.abs().sum(1))
+
+
 def test_lookup_grad_of_nothing():
     g = gen(1)
     for ids in (torch.empty(0, dtype=torch.int32, device="cuda"), torch.full((70,), -1, device="cuda")):
@@ -257,6 +272,14 @@ def test_lookup_grad_strides_and_alignments():
         # another alignment may add in another order: held to the definition
         lookup_grad_check(wide[..., a:b].reshape(900, -1), ids, 40, None, 1.0, buf[:, 7:7 + b - a])
         assert bool((buf[:, :7] == 9).all()) and bool((buf[:, 7 + b - a:] == 9).all())
+        wide_out = torch.full((40, 230), 9.0, device="cuda")  # in 32 bits, at odd places
+        tokens.lookup_grad(wide[..., a:b], p, out=wide_out[:, 3:3 + b - a])
+        lookup_grad_check(wide[..., a:b].reshape(900, -1), ids, 40, None, 1.0, wide_out[:, 3:3 + b - a])
+        assert bool((wide_out[:, :3] == 9).all()) and bool((wide_out[:, 3 + b - a:] == 9).all())
+        base = normal(g, 40, b - a, dtype=F16)  # added to, in 16 bits
+        acc = base.clone()
+        tokens.lookup_grad(wide[..., a:b], p, out=acc, accumulate=True)
+        lookup_grad_check(wide[..., a:b].reshape(900, -1), ids, 40, None, 1.0, acc, base)
     one = normal(g, 1, 64)
     dt = tokens.lookup_grad(one.expand(900, 64), p)  # a broadcast gradient
     lookup_grad_check(one.expand(900, 64), ids, 40, None, 1.0, dt)
@@ -386,6 +409,33 @@ def test_group_strides_and_alignments():
             within(dw, prod.sum(2), 1.001 * (b - a + 2) * U32 * prod.abs().sum(2))
     one = normal(g, 1, 64)
     assert torch.equal(tokens.group(one.expand(90, 64), p)[:valid], one.expand(valid, 64))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,columns,dim", [(40_000, 2, 64), (40_000, 1, 64), (30_000, 4, 16), (20_000, 8, 32), (70_001, 2, 8),
+                                           (3000, 3, 1024), (9000, 12, 64)])
+def test_group_of_many_tokens(dtype, n, columns, dim):
+    # enough for every launch shape that large batches take
+    g = gen(n + columns)
+    ids = make_ids(g, (n, columns), 300, pad=0.05)
+    p = tokens.plan(ids, 300)
+    slot = p.slot.long()
+    ok, at = slot >= 0, slot.clamp(min=0)
+    x, rows = normal(g, n, dim, dtype=dtype), normal(g, n * columns, dim, dtype=dtype)
+    w = torch.rand(n, columns, generator=g, device="cuda")
+    want = (x.double()[:, None, :] * w.double()[..., None])[ok]
+    within(tokens.group(x, p, weights=w)[slot[ok]], want, (U[dtype] + U32) * want.abs() + TINY[dtype])
+    dxs, dw = tokens.ungroup_grad(x, p, weights=w, xs=rows)
+    within(dxs[slot[ok]], want, (U[dtype] + U32) * want.abs() + TINY[dtype])
+    picked = rows.double()[at].masked_fill(~ok[..., None], 0.0)
+    prod = picked * x.double()[:, None, :]
+    within(dw, prod.sum(2), 1.001 * (dim + 2) * U32 * prod.abs().sum(2))
+    terms = picked * w.double()[..., None]
+    want, tol = terms.sum(1), 1.001 * (columns + 2) * U32 * terms.abs().sum(1)
+    within(tokens.ungroup(rows, p, weights=w), want, tol + U[dtype] * (want.abs() + tol) + TINY[dtype])
+    dx, dw2 = tokens.group_grad(rows, p, weights=w, x=x)
+    within(dx, want, tol + U[dtype] * (want.abs() + tol) + TINY[dtype])
+    within(dw2, prod.sum(2), 1.001 * (dim + 2) * U32 * prod.abs().sum(2))
 
 
 def test_group_of_nothing():
