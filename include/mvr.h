@@ -680,7 +680,7 @@ int mvr_normalize_rows_device(mvr_ctx* ctx, float* d_rows, uint64_t n_floats, ui
  *
  * Rows have `dim` elements of one type (mvr_dtype), consecutive inside a row;
  * `*_stride` is the distance of two rows in elements (at least dim for
- * outputs, any value for inputs: 0 repeats one row). Scales and weights are
+ * outputs, any value for inputs: 0 repeats one row; below 2^32). Scales and weights are
  * f32. Sums and products are formed in f32 and rounded once to the element
  * type. Results do not depend on the launch: the order of every sum is fixed
  * by the sizes.

@@ -93,7 +93,8 @@ struct GradShape {
   uint32_t tiles;
   uint32_t dots;       // blocks behind them for dscale, where a row's parts lie in several blocks
   uint32_t fill_lanes;  // lanes of a row there, a power of two
-  uint64_t gs, ts, ds;  // row strides of grad, table, dtable
+  uint32_t gs, ts;  // row strides of grad and table
+  uint64_t ds;      // of dtable
 };
 
 template <class T, class O, int V>
@@ -154,8 +155,8 @@ __device__ __forceinline__ void scale_dots(const GradArgs<T, O, V>& A) {
   if (i >= S.n) return;
   float dot = 0.f;
   if (r < S.rows) {
-    const T* a = A.grad + i * S.gs;
-    const T* b = A.table + r * S.ts;
+    const T* a = A.grad + (uint64_t)i * S.gs;
+    const T* b = A.table + (uint64_t)r * S.ts;
     for (uint32_t c0 = lane; c0 < chunks; c0 += U * 32) {
       Raw<T, V> x[U], y[U];
 #pragma unroll
@@ -286,11 +287,19 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
   uint32_t cur = a < b ? s_key[a] : S.rows;
   uint32_t hkind = 0;
   Raw<T, V> trow[NCH];  // the table's row of `cur`
-  auto load_row = [&](Raw<T, V> (&r)[NCH], const T* base, uint64_t at, bool in) {
+  const T* grad[NCH];
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) grad[k] = A.grad + col[k];
+  auto load_grad = [&](Raw<T, V> (&r)[NCH], uint32_t token) {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+      if (on[k]) r[k].load(grad[k] + (uint64_t)token * S.gs);
+  };
+  auto load_table = [&](Raw<T, V> (&r)[NCH], uint32_t key) {
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       r[k].zero();
-      if (in && on[k]) r[k].load(base + at + col[k]);
+      if (key < S.rows && on[k]) r[k].load(A.table + (uint64_t)key * S.ts + col[k]);
     }
   };
   auto add = [&](const Raw<T, V> (&r)[NCH], float f) {
@@ -307,19 +316,23 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
       for (int v = 0; v < V; ++v) d = fmaf(x[k].get(v), y[k].get(v), d);
     return d;
   };
-  if constexpr (DSCALE) load_row(trow, A.table, cur * S.ts, cur < S.rows);
+  if constexpr (DSCALE) load_table(trow, cur);
 
-  Raw<T, V> row[U][NCH];
+  Raw<T, V> row[U][NCH];  // zeros for good where the lane is behind the row's end
   float f[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) row[u][k].zero();
   auto load_step = [&](uint32_t p0) {  // groups begin at multiples of 8 places
 #pragma unroll
     for (int u = 0; u < U; u += 4) {
       if (p0 + u >= b) break;
       const uint4 t = *reinterpret_cast<const uint4*>(s_tok + p0 + u);
-      load_row(row[u], A.grad, t.x * S.gs, true);
-      load_row(row[u + 1], A.grad, t.y * S.gs, p0 + u + 1 < b);
-      load_row(row[u + 2], A.grad, t.z * S.gs, p0 + u + 2 < b);
-      load_row(row[u + 3], A.grad, t.w * S.gs, p0 + u + 3 < b);
+      load_grad(row[u], t.x);
+      if (p0 + u + 1 < b) load_grad(row[u + 1], t.y);
+      if (p0 + u + 2 < b) load_grad(row[u + 2], t.z);
+      if (p0 + u + 3 < b) load_grad(row[u + 3], t.w);
       const float4 x = *reinterpret_cast<const float4*>(s_scale + p0 + u);
       f[u] = x.x;
       f[u + 1] = x.y;
@@ -349,8 +362,7 @@ lookup_grad_tile_kernel(const GradArgs<T, O, V> A) {
         Raw<T, V> other[U][NCH];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const uint32_t key = p0 + u < b ? s_key[p0 + u] : S.rows;
-          load_row(other[u], A.table, key * S.ts, key < S.rows);
+          load_table(other[u], p0 + u < b ? s_key[p0 + u] : S.rows);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) dot[u] = times(row[u], other[u]);
@@ -607,7 +619,7 @@ int mvr_lookup_grad_device(mvr_ctx* h, const void* d_grad, int dtype, uint64_t g
       return mvr::tok::by_vec<T>(w, [&](auto vec) {
         constexpr int V = decltype(vec)::value;
         mvr::tok::GradArgs<T, O, V> A;
-        A.s = {n, v, dim, 0, 0, 0, 0, 0, 0, grad_stride, table_stride, dtable_stride};
+        A.s = {n, v, dim, 0, 0, 0, 0, 0, 0, (uint32_t)grad_stride, (uint32_t)table_stride, dtable_stride};
         A.grad = (const T*)d_grad;
         A.offsets = d_offsets;
         A.order = d_order;

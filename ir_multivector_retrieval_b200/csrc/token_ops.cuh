@@ -296,6 +296,7 @@ inline int check_rows(Ctx* c, const char* what, const void* p, int dtype, uint64
   if (n > kMaxElems / dim) return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + ": more than 2^38 elements");
   if (!aligned(p, elem_size(dtype)))
     return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + " is not aligned to its element type");
+  if (stride >> 32) return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + ": stride above 2^32 - 1");
   if (output && stride < dim) return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + ": stride below dim");
   return MVR_OK;
 }

@@ -684,7 +684,7 @@ def test_c_entry_refusals(ctx):
 
     assert lookup() == 0
     for kw in (dict(table=None), dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=2**31 - 1), dict(ids=None),
-               dict(idb=2), dict(ids=j + 2), dict(idb=8, ids=j + 4), dict(out=None), dict(os=7), dict(table=a + 2),
+               dict(idb=2), dict(ids=j + 2), dict(idb=8, ids=j + 4), dict(out=None), dict(os=7), dict(os=2**32), dict(ts=2**32), dict(table=a + 2),
                dict(out=a + 4098), dict(scale=a + 1)):
         assert lookup(**kw) == bad, kw
     assert lookup(d=0) == dim and lookup(n=0, ids=None, out=None) == 0
