@@ -1,11 +1,12 @@
 /*
  * mvr.h — C ABI of the B200 build path for the TAC multivector index:
  * PQ codebook training, PQ encoding, the shared k-means primitive and
- * TAC per-token clustering.
+ * TAC per-token clustering; and token operators of language models: a table
+ * read by token id and rows sorted by group, with their gradients.
  *
- * Every entry point replaces one function of the reference Zig build path
- * (BleedingDev/ir-multivector-retrieval). The citation beside each
- * declaration names the reference function it stands in for, as
+ * Every entry point but the token operators (at the end) replaces one function
+ * of the reference Zig build path (BleedingDev/ir-multivector-retrieval). The
+ * citation beside each declaration names the reference function it stands in for, as
  * `path:line` inside that project. A Zig host binds these symbols with
  * `@cImport(@cInclude("mvr.h"))` and keeps its own signatures.
  *

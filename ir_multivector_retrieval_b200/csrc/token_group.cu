@@ -15,7 +15,9 @@ namespace {
 // the dot products.
 
 // dst[slot[i, c]] = w[i, c] * src[i]: a token's row is read once. KU choices'
-// places are asked for at once, beside the rows.
+// places are asked for at once, beside the rows. 1,521,797 x 2 choices x 64
+// f32: 187 us (6.3 TB/s; 215 us with 16 bytes a lane, 222 us with the places
+// read one after the other).
 template <class T, int V, int UR, int KU>
 __global__ void __launch_bounds__(256)
 spread_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
@@ -60,7 +62,9 @@ spread_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, 
   }
 }
 
-// dst[i] = sum_c w[i, c] * src[slot[i, c]]: KU choices' rows in flight.
+// dst[i] = sum_c w[i, c] * src[slot[i, c]]: KU choices' rows in flight, four at
+// most (4093 x 8 x 2048 f16: 26 us, with eight 28). 1,521,797 x 2 x 64 f32: 185
+// us (6.3 TB/s; 230 us with 16 bytes a lane).
 template <class T, int V, int KU>
 __global__ void __launch_bounds__(256)
 collect_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns, uint64_t pairs,
@@ -103,6 +107,8 @@ collect_kernel(Flat F, const T* __restrict__ src, uint64_t ss, uint32_t columns,
 // other[slot]>. A group of L lanes has a pair, so a token's row is read once
 // from memory and again from the caches for its other choices. Rows that L
 // lanes hold at once are taken PU at a time, longer ones CU chunks at a time.
+// 8192 x 8 x 2048 bf16: 88 us (6.4 TB/s); 1,521,797 x 2 x 64 f32: 312 us (6.2
+// TB/s; 800 us with one pair at a time).
 template <class T, int V, int PU, int CU, bool DST>
 __global__ void __launch_bounds__(256)
 spread_dot_kernel(uint32_t L, uint32_t chunks, const T* __restrict__ src, uint64_t ss, uint32_t columns,
