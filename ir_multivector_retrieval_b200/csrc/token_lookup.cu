@@ -188,7 +188,7 @@ __device__ __forceinline__ void scale_dots(const GradArgs<T, O, V>& A) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-  if (lane == 0) A.dscale[i] = A.alpha * dot;
+  if (lane == 0) A.dscale[i] = r < S.rows ? A.alpha * dot : 0.f;
 }
 
 // Places of a tile whose plan entries a block keeps in shared memory.

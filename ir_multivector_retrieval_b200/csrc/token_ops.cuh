@@ -1,4 +1,4 @@
-// token_ops.cuh — what the token operators share: rows read up to 16 bytes a
+// token_ops.cuh — what the token operators share: rows read up to 32 bytes a
 // lane, work numbered through rows, argument checks and dispatch by element
 // type and width.
 #pragma once
@@ -20,7 +20,7 @@ namespace tok {
 
 constexpr uint32_t kNoSlot = MVR_NO_SLOT;
 constexpr uint64_t kMaxIds = 0x7FFFFFFFull;   // pairs of a plan: places fit 31 bits
-constexpr uint64_t kMaxElems = 1ull << 38;
+constexpr uint64_t kMaxElems = 1ull << 38;    // of one tensor: fewer than 2^31 blocks of 256 threads
 constexpr uint64_t kMaxRows = 0x7FFFFFFEull;  // rows + 1 offsets, and `rows` itself is the key of no row
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -286,13 +286,12 @@ inline int check_ids(Ctx* c, const void* ids, int id_bytes, uint64_t n, uint64_t
   return MVR_OK;
 }
 
-inline int check_rows(Ctx* c, const char* what, const void* p, int dtype, uint64_t n, uint32_t dim, uint64_t stride,
-               bool output) {
+inline int check_rows(Ctx* c, const char* what, const void* p, int dtype, uint64_t n, uint32_t dim,
+                      uint64_t stride, bool output) {
   if (!known(dtype)) return bad(c, "unknown element type");
   if (dim == 0) return fail(c, MVR_E_DIM_MISMATCH, "dim == 0");
   if (dim > MVR_MAX_ROW_DIM) return bad(c, "dim above MVR_MAX_ROW_DIM");
   if (n && !p) return fail(c, MVR_E_INVALID_ARGUMENT, std::string("null pointer: ") + what);
-  // what one launch covers: 2^31 - 1 blocks of 256 elements
   if (n > kMaxElems / dim) return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + ": more than 2^38 elements");
   if (!aligned(p, elem_size(dtype)))
     return fail(c, MVR_E_INVALID_ARGUMENT, std::string(what) + " is not aligned to its element type");

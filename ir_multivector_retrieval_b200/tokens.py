@@ -78,7 +78,7 @@ def _rows(t, what: str, n: int | None = None, dim: int | None = None):
     if one != 1 and d > 1:
         t = t.contiguous()
         stride = d
-    return t, d, stride
+    return t, d, stride if m > 1 else d
 
 
 def _out_rows(t, what: str, n: int, dim: int, dtype):
@@ -98,7 +98,7 @@ def _out_rows(t, what: str, n: int, dim: int, dtype):
     stride, one = t.stride()
     if dim > 1 and one != 1 or n > 1 and stride < dim:
         _refuse(f"{what} must have consecutive, separate rows")
-    return t.data_ptr(), stride if n > 1 else max(stride, dim)
+    return t.data_ptr(), stride if n > 1 else dim
 
 
 def _f32(t, n: int, what: str):

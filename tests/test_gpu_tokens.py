@@ -257,6 +257,28 @@ def test_lookup_grad_of_padding_reads_no_gradient():
     assert torch.equal(dt, wt) and torch.equal(ds, ws) and bool((ds[100:200] == 0).all())
 
 
+@pytest.mark.parametrize("dim", [16, 64, 700])
+def test_padding_has_no_gradient_whatever_the_constant(dim):
+    g = gen(dim)
+    ids = make_ids(g, (60,), 7)
+    ids[::3] = -1
+    p = tokens.plan(ids, 7)
+    dt, ds = tokens.lookup_grad(normal(g, 60, dim), p, alpha=float("inf"), table=normal(g, 7, dim))
+    assert bool((ds[::3] == 0).all()) and not torch.isfinite(ds[ids >= 0]).any()
+    out = tokens.lookup(normal(g, 7, dim), ids, alpha=float("inf"))
+    assert bool((out[::3] == 0).all())
+
+
+def test_one_row_has_any_stride():
+    x = torch.arange(8.0, device="cuda")
+    row = x.as_strided((1, 8), (2**40, 1))
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    p = tokens.plan(zero, 1)
+    out = torch.zeros(8, device="cuda").as_strided((1, 8), (2**40, 1))
+    for r in (tokens.lookup(row, zero, out=out), tokens.lookup_grad(row, p), tokens.group(row, p), tokens.ungroup(row, p)):
+        assert torch.equal(r.view(-1), x)
+
+
 def test_lookup_grad_strides_and_alignments():
     g = gen(4)
     ids = make_ids(g, (3, 300), 40, spread="head")
@@ -684,7 +706,8 @@ def test_c_entry_refusals(ctx):
 
     assert lookup() == 0
     for kw in (dict(table=None), dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=2**31 - 1), dict(ids=None),
-               dict(idb=2), dict(ids=j + 2), dict(idb=8, ids=j + 4), dict(out=None), dict(os=7), dict(os=2**32), dict(ts=2**32), dict(table=a + 2),
+               dict(idb=2), dict(ids=j + 2), dict(idb=8, ids=j + 4), dict(out=None), dict(os=7), dict(os=2**32),
+               dict(ts=2**32), dict(d=2**20 + 1, os=2**21), dict(n=2**40), dict(table=a + 2),
                dict(out=a + 4098), dict(scale=a + 1)):
         assert lookup(**kw) == bad, kw
     assert lookup(d=0) == dim and lookup(n=0, ids=None, out=None) == 0
