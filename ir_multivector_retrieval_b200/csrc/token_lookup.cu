@@ -530,14 +530,19 @@ int lookup_grad_run(Ctx* c, GradArgs<T, O, V> A) {
   S.lanes = std::min(32u, pow2_ceil((chunks + NCH - 1) / NCH));
   const uint32_t slabs = (chunks + S.lanes * NCH - 1) / (S.lanes * NCH);
   const uint32_t groups = 256 / S.lanes;
-  // Long groups leave fewer sums to join, short ones more blocks: the longest
-  // of 8 to 64 places that still gives every SM eight blocks, as long as the
-  // tile's plan fits.
-  S.per_group = std::min(64u, kMaxTile / groups);
-  while (S.per_group > 8 &&
-         (uint64_t)slabs * ((S.n + (uint64_t)groups * S.per_group - 1) / ((uint64_t)groups * S.per_group)) <
-             8ull * c->sm_count)
-    S.per_group >>= 1;
+  // Few places are one tile, which leaves nothing to join: four steps of a group
+  // take no longer than another launch. Otherwise long groups leave fewer sums
+  // to join, short ones more blocks: the longest of 8 to 64 places that still
+  // gives every SM eight blocks, as long as the tile's plan fits.
+  const uint32_t most = kMaxTile / groups;
+  S.per_group = (S.n / groups + 8) / 8 * 8;
+  if (S.per_group > std::min(16u, most)) {
+    S.per_group = std::min(64u, most);
+    while (S.per_group > 8 &&
+           (uint64_t)slabs * ((S.n + (uint64_t)groups * S.per_group - 1) / ((uint64_t)groups * S.per_group)) <
+               8ull * c->sm_count)
+      S.per_group >>= 1;
+  }
   const uint32_t tile = groups * S.per_group;
   S.tiles = (uint32_t)((S.n + (uint64_t)tile - 1) / tile);
   S.fill_lanes = std::min(32u, pow2_ceil(chunks));

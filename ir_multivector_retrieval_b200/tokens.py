@@ -18,43 +18,33 @@ import atexit
 import ctypes as C
 import functools
 import threading
-from contextlib import nullcontext
 from dataclasses import dataclass
+
+import torch
 
 from . import _lib
 from ._lib import CODES, MvrError
 
 MAX_IDS = 2**31 - 1
 
+_F32, _I32 = torch.float32, torch.int32
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # mvr_dtype
+_ID_BYTES = {torch.int32: 4, torch.uint32: 4, torch.int64: 8}
+
 
 def _refuse(msg: str, name: str = "InvalidArgument"):
     raise MvrError(CODES[name], msg)
 
 
-@functools.cache
-def _torch():
-    import torch
-
-    return torch
-
-
-@functools.cache
-def _types() -> dict:
-    """Element types (mvr_dtype) and id types (bytes) by torch type."""
-    torch = _torch()
-    return {"rows": {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2},
-            "ids": {torch.int32: 4, torch.uint32: 4, torch.int64: 8}, "f32": torch.float32, "i32": torch.int32}
-
-
 def _dtype(t, what: str) -> int:
-    d = _types()["rows"].get(getattr(t, "dtype", None))
+    d = _ROW_TYPES.get(getattr(t, "dtype", None))
     if d is None:
         _refuse(f"{what} must be a float32, bfloat16 or float16 tensor, not {getattr(t, 'dtype', type(t))}")
     return d
 
 
 def _id_bytes(ids) -> int:
-    n = _types()["ids"].get(getattr(ids, "dtype", None))
+    n = _ID_BYTES.get(getattr(ids, "dtype", None))
     if n is None:
         _refuse(f"ids must be an int32, int64 or uint32 tensor, not {getattr(ids, 'dtype', type(ids))}")
     return n
@@ -102,24 +92,21 @@ def _out_rows(t, what: str, n: int, dim: int, dtype):
 
 
 def _f32(t, n: int, what: str):
-    if t.dtype != _types()["f32"]:
+    if t.dtype != _F32:
         _refuse(f"{what} must be float32, not {t.dtype}")
     if t.numel() != n:
         _refuse(f"{what} has {t.numel()} values, not {n}", "LengthMismatch")
     return t if t.is_contiguous() else t.contiguous()
 
 
-@functools.cache
-def _raw_stream():
-    torch = _torch()
-    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-        lambda device: torch.cuda.current_stream(device).cuda_stream)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _stream_of(device: int) -> int:
     """Handle of torch's current stream; 1 names the legacy default stream,
     whose own handle, 0, would select a context's own stream."""
-    return _raw_stream()(device) or 1
+    return _raw_stream(device) or 1
 
 
 class _Follower:
@@ -154,30 +141,29 @@ def _follower(device: int) -> _Follower:
     return f
 
 
-def _run(ctx, device: int, call):
-    """`call(lib, handle)` on the right context and stream, its status checked.
-    Contexts are not for two calls at once, hence the locks."""
+def _run(ctx, device: int, name: str, *args):
+    """The library's `name` on the right context and stream, its status
+    checked. Contexts are not for two calls at once, hence the locks."""
     if ctx is None:
-        f = _follower(device)
+        f = _followers.get(device) or _follower(device)
         ctx = f.ctx
         with ctx.lock:
-            here = _stream_of(device)
+            here = _raw_stream(device) or 1
             if f.at != here:
                 ctx.lib.mvr_ctx_set_stream(ctx.handle, here)
                 f.at = here
-            status = call(ctx.lib, ctx.handle)
+            status = getattr(ctx.lib, name)(ctx.handle, *args)
             if status:
                 ctx.check(status)
         return
     if ctx.device != device:
         _refuse(f"tensors on device {device}, context on device {ctx.device}")
     with ctx.lock:
-        here = _stream_of(device)
         own = ctx.stream == 0
         if own:
-            ctx.lib.mvr_ctx_set_stream(ctx.handle, here)
+            ctx.lib.mvr_ctx_set_stream(ctx.handle, _stream_of(device))
         try:
-            status = call(ctx.lib, ctx.handle)
+            status = getattr(ctx.lib, name)(ctx.handle, *args)
             if status:
                 ctx.check(status)
         finally:
@@ -185,33 +171,40 @@ def _run(ctx, device: int, call):
                 ctx.lib.mvr_ctx_set_stream(ctx.handle, None)
 
 
-def _place(ctx, *tensors):
-    """The GPU that all the tensors lie on, and the scope in which results and
-    copies are made: nothing to do on torch's current stream. With a stream
-    given to ``ctx.set_stream`` they come from that stream's memory pool, and
-    the inputs stay alive for it."""
+def _device_of(*tensors) -> int:
+    """The GPU that all the tensors lie on."""
     device = -1
     for t in tensors:
         if t is None:
             continue
-        if not getattr(t, "is_cuda", False):
+        d = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if d < 0:
             _refuse("all tensors must be CUDA tensors (there is no CPU fallback)")
-        d = t.get_device()
-        if device < 0:
+        if d != device:
+            if device >= 0:
+                _refuse(f"tensors on devices {device} and {d}")
             device = d
-        elif d != device:
-            _refuse(f"tensors on devices {device} and {d}")
-    if ctx is None or ctx.stream == 0 or ctx.stream == _stream_of(device):
-        return device, _here
-    torch = _torch()
-    s = torch.cuda.ExternalStream(ctx.stream, device=device)
-    for t in tensors:
-        if t is not None:
-            t.record_stream(s)
-    return device, torch.cuda.stream(s)
+    return device
 
 
-_here = nullcontext()
+def _on_its_stream(call):
+    """With a stream given to ``ctx.set_stream`` that is not torch's current
+    one, results and copies come from that stream's memory pool, and the
+    inputs stay alive for it."""
+
+    @functools.wraps(call)
+    def wrapped(*args, ctx=None, **kw):
+        if ctx is None or ctx.stream == 0 or ctx.stream == _stream_of(ctx.device):
+            return call(*args, ctx=ctx, **kw)
+        s = torch.cuda.ExternalStream(ctx.stream, device=ctx.device)
+        for t in (*args, *kw.values()):
+            for u in (t.offsets, t.order, t.keys, t.slot) if isinstance(t, Plan) else (t,):
+                if isinstance(u, torch.Tensor) and u.is_cuda:
+                    u.record_stream(s)
+        with torch.cuda.stream(s):
+            return call(*args, ctx=ctx, **kw)
+
+    return wrapped
 
 
 @dataclass
@@ -243,12 +236,12 @@ class Plan:
         return self.slot.numel() // s[-1] if len(s) > 1 and s[-1] else s[0] if len(s) == 1 else 0
 
     def _check(self):
-        i32 = _types()["i32"]
-        for t in (self.offsets, self.order, self.keys, self.slot):
-            if t.dtype != i32 or not t.is_contiguous():
-                _refuse("a plan's tensors must be contiguous int32 tensors")
-        n = self.slot.numel()
-        if self.offsets.numel() != self.rows + 1 or self.order.numel() != n or self.keys.numel() != n:
+        offsets, order, keys, slot = self.offsets, self.order, self.keys, self.slot
+        if not (offsets.dtype == order.dtype == keys.dtype == slot.dtype == _I32 and offsets.is_contiguous()
+                and order.is_contiguous() and keys.is_contiguous() and slot.is_contiguous()):
+            _refuse("a plan's tensors must be contiguous int32 tensors")
+        n = slot.numel()
+        if offsets.numel() != self.rows + 1 or order.numel() != n or keys.numel() != n:
             _refuse("plan: sizes differ", "LengthMismatch")
         return n
 
@@ -272,41 +265,41 @@ def _grad_bytes(n: int, dim: int) -> int:
 
 
 def _workspace(like, need: int):
-    return like.new_empty(need, dtype=_torch().uint8) if need else None
+    return like.new_empty(need, dtype=torch.uint8) if need else None
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+@_on_its_stream
 def plan(ids, rows: int, *, ctx=None) -> Plan:
     """Sort the ids ([n] or [n, columns]) by value, stable."""
     rows = int(rows)
     if not 0 < rows < MAX_IDS:
         _refuse(f"rows must be in [1, 2^31 - 2], not {rows}")
     idb = _id_bytes(ids)
-    if ids.dim() not in (1, 2):
+    dims = ids.dim()
+    if dims not in (1, 2):
         _refuse("ids must have one or two dimensions")
-    if ids.dim() == 2 and ids.shape[1] == 0:
+    if dims == 2 and ids.shape[1] == 0:
         _refuse("ids have no columns")
     n = ids.numel()
     if n > MAX_IDS:
         _refuse("more than 2^31 - 1 ids")
-    device, scope = _place(ctx, ids)
-    with scope:
-        ids = ids.contiguous()
-        i32 = _types()["i32"]
-        offsets, order, keys, slot = ids.new_empty(rows + 1 + 3 * n, dtype=i32).split((rows + 1, n, n, n))
-        if ids.dim() == 2:
-            slot = slot.view(ids.shape)
-        need = _plan_bytes(n, rows)
-        ws = _workspace(ids, need)
-        _run(ctx, device, lambda lib, h: lib.mvr_token_plan_device(
-            h, ids.data_ptr(), idb, n, rows, offsets.data_ptr(), order.data_ptr(), keys.data_ptr(), slot.data_ptr(),
-            _ptr(ws), need))
+    device = _device_of(ids)
+    ids = ids.contiguous()
+    offsets, order, keys, slot = ids.new_empty(rows + 1 + 3 * n, dtype=_I32).split((rows + 1, n, n, n))
+    if dims == 2:
+        slot = slot.view(ids.shape)
+    need = _plan_bytes(n, rows)
+    ws = _workspace(ids, need)
+    _run(ctx, device, "mvr_token_plan_device", ids.data_ptr(), idb, n, rows, offsets.data_ptr(), order.data_ptr(),
+         keys.data_ptr(), slot.data_ptr(), _ptr(ws), need)
     return Plan(rows, offsets, order, keys, slot)
 
 
+@_on_its_stream
 def lookup(table, ids, *, scale=None, alpha: float = 1.0, out=None, ctx=None):
     """``out[i] = (alpha * scale[i]) * table[ids[i]]``: the ids' shape plus the
     table's row length, in the table's type; zero rows where an id names none.
@@ -316,23 +309,23 @@ def lookup(table, ids, *, scale=None, alpha: float = 1.0, out=None, ctx=None):
     n = ids.numel()
     if table.dim() != 2:
         _refuse("table must have two dimensions", "DimMismatch")
-    device, scope = _place(ctx, table, ids, scale, out)
-    with scope:
-        rows = table.shape[0]
-        t, dim, ts = _rows(table, "table")
-        ids_ = ids.contiguous()
-        if scale is not None:
-            scale = _f32(scale, n, "scale")
-        if out is None:
-            out = t.new_empty((*ids.shape, dim))
-            po, so = out.data_ptr(), dim
-        else:
-            po, so = _out_rows(out, "out", n, dim, t.dtype)
-        _run(ctx, device, lambda lib, h: lib.mvr_lookup_device(
-            h, t.data_ptr(), dt, rows, dim, ts, ids_.data_ptr(), idb, n, _ptr(scale), alpha, po, so))
+    device = _device_of(table, ids, scale, out)
+    rows = table.shape[0]
+    table, dim, ts = _rows(table, "table")
+    flat = ids.contiguous()
+    if scale is not None:
+        scale = _f32(scale, n, "scale")
+    if out is None:
+        out = table.new_empty((*ids.shape, dim))
+        po, so = out.data_ptr(), dim
+    else:
+        po, so = _out_rows(out, "out", n, dim, table.dtype)
+    _run(ctx, device, "mvr_lookup_device", table.data_ptr(), dt, rows, dim, ts, flat.data_ptr(), idb, n, _ptr(scale),
+         alpha, po, so)
     return out
 
 
+@_on_its_stream
 def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None, out=None, accumulate: bool = False,
                 ctx=None):
     """Gradients of ``lookup`` from that of its output (the ids' shape plus the
@@ -347,32 +340,30 @@ def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None,
     rows = plan.rows
     if accumulate and out is None:
         _refuse("accumulate needs out")
-    device, scope = _place(ctx, grad, plan.offsets, plan.order, plan.keys, plan.slot, scale, table, out)
-    with scope:
-        g, dim, gs = _rows(grad, "grad", n)
-        if scale is not None:
-            scale = _f32(scale, n, "scale")
-        tp, ts, dscale = None, dim, None
-        if table is not None:
-            if table.dtype != g.dtype:
-                _refuse(f"table is {table.dtype}, grad {g.dtype}")
-            table, _, ts = _rows(table, "table", rows, dim)
-            tp = table.data_ptr()
-            dscale = g.new_empty(plan.slot.shape, dtype=_types()["f32"])
-        if out is None:
-            out = g.new_empty((rows, dim))
-            po, so, odt = out.data_ptr(), dim, dt
-        else:
-            odt = _dtype(out, "out")
-            if odt not in (dt, 0):
-                _refuse("out must have grad's type or float32")
-            po, so = _out_rows(out, "out", rows, dim, out.dtype)
-        need = _grad_bytes(n, dim)
-        ws = _workspace(g, need)
-        _run(ctx, device, lambda lib, h: lib.mvr_lookup_grad_device(
-            h, g.data_ptr(), dt, gs, n, rows, dim, plan.offsets.data_ptr(), plan.order.data_ptr(),
-            plan.keys.data_ptr(), _ptr(scale), alpha, tp, ts, po, odt, so, int(accumulate),
-            _ptr(dscale), _ptr(ws), need))
+    device = _device_of(grad, plan.offsets, plan.order, plan.keys, plan.slot, scale, table, out)
+    grad, dim, gs = _rows(grad, "grad", n)
+    if scale is not None:
+        scale = _f32(scale, n, "scale")
+    tp, ts, dscale = None, dim, None
+    if table is not None:
+        if table.dtype != grad.dtype:
+            _refuse(f"table is {table.dtype}, grad {grad.dtype}")
+        table, _, ts = _rows(table, "table", rows, dim)
+        tp = table.data_ptr()
+        dscale = grad.new_empty(plan.slot.shape, dtype=_F32)
+    if out is None:
+        out = grad.new_empty((rows, dim))
+        po, so, odt = out.data_ptr(), dim, dt
+    else:
+        odt = _dtype(out, "out")
+        if odt not in (dt, 0):
+            _refuse("out must have grad's type or float32")
+        po, so = _out_rows(out, "out", rows, dim, out.dtype)
+    need = _grad_bytes(n, dim)
+    ws = _workspace(grad, need)
+    _run(ctx, device, "mvr_lookup_grad_device", grad.data_ptr(), dt, gs, n, rows, dim, plan.offsets.data_ptr(),
+         plan.order.data_ptr(), plan.keys.data_ptr(), _ptr(scale), alpha, tp, ts, po, odt, so, int(accumulate),
+         _ptr(dscale), _ptr(ws), need)
     return out if dscale is None else (out, dscale)
 
 
@@ -380,18 +371,17 @@ def _token_call(name: str, src, what: str, from_n: int, plan: Plan, weights, to_
     """group and ungroup: rows of `src` to rows of `out`."""
     dt = _dtype(src, what)
     n_ids = plan._check()
-    device, scope = _place(ctx, src, plan.slot, weights, out)
-    with scope:
-        s, dim, ss = _rows(src, what, from_n)
-        if weights is not None:
-            weights = _f32(weights, n_ids, "weights")
-        if out is None:
-            out = s.new_empty((to_n, dim))
-            po, so = out.data_ptr(), dim
-        else:
-            po, so = _out_rows(out, "out", to_n, dim, s.dtype)
-        _run(ctx, device, lambda lib, h: getattr(lib, name)(
-            h, s.data_ptr(), dt, ss, plan.n, plan.columns, dim, plan.slot.data_ptr(), _ptr(weights), po, so))
+    slot = plan.slot
+    device = _device_of(src, slot, weights, out)
+    src, dim, ss = _rows(src, what, from_n)
+    if weights is not None:
+        weights = _f32(weights, n_ids, "weights")
+    if out is None:
+        out = src.new_empty((to_n, dim))
+        po, so = out.data_ptr(), dim
+    else:
+        po, so = _out_rows(out, "out", to_n, dim, src.dtype)
+    _run(ctx, device, name, src.data_ptr(), dt, ss, plan.n, plan.columns, dim, slot.data_ptr(), _ptr(weights), po, so)
     return out
 
 
@@ -400,29 +390,29 @@ def _token_grad(name: str, src, from_n: int, plan: Plan, weights, other, other_w
     """Their gradients: also the weights' where the forward rows are given."""
     dt = _dtype(src, "dout")
     n_ids = plan._check()
-    device, scope = _place(ctx, src, plan.slot, weights, other, out)
-    with scope:
-        s, dim, ss = _rows(src, "dout", from_n)
-        if weights is not None:
-            weights = _f32(weights, n_ids, "weights")
-        dw, op, os_ = None, None, dim
-        if other is not None:
-            if other.dtype != s.dtype:
-                _refuse(f"{other_what} is {other.dtype}, dout {s.dtype}")
-            other, _, os_ = _rows(other, other_what, other_n, dim)
-            op = other.data_ptr()
-            dw = s.new_empty(plan.slot.shape, dtype=_types()["f32"])
-        if out is None:
-            out = s.new_empty((to_n, dim))
-            po, so = out.data_ptr(), dim
-        else:
-            po, so = _out_rows(out, "out", to_n, dim, s.dtype)
-        _run(ctx, device, lambda lib, h: getattr(lib, name)(
-            h, s.data_ptr(), dt, ss, plan.n, plan.columns, dim, plan.slot.data_ptr(), _ptr(weights), op, os_, po, so,
-            _ptr(dw)))
+    slot = plan.slot
+    device = _device_of(src, slot, weights, other, out)
+    src, dim, ss = _rows(src, "dout", from_n)
+    if weights is not None:
+        weights = _f32(weights, n_ids, "weights")
+    dw, op, os_ = None, None, dim
+    if other is not None:
+        if other.dtype != src.dtype:
+            _refuse(f"{other_what} is {other.dtype}, dout {src.dtype}")
+        other, _, os_ = _rows(other, other_what, other_n, dim)
+        op = other.data_ptr()
+        dw = src.new_empty(slot.shape, dtype=_F32)
+    if out is None:
+        out = src.new_empty((to_n, dim))
+        po, so = out.data_ptr(), dim
+    else:
+        po, so = _out_rows(out, "out", to_n, dim, src.dtype)
+    _run(ctx, device, name, src.data_ptr(), dt, ss, plan.n, plan.columns, dim, slot.data_ptr(), _ptr(weights), op, os_,
+         po, so, _ptr(dw))
     return out if dw is None else (out, dw)
 
 
+@_on_its_stream
 def group(x, plan: Plan, *, weights=None, out=None, ctx=None):
     """The rows of x (one a token) in sorted order: ``out[slot[i, c]] =
     weights[i, c] * x[i]``, n * columns rows. Rows behind the last sorted one
@@ -430,6 +420,7 @@ def group(x, plan: Plan, *, weights=None, out=None, ctx=None):
     return _token_call("mvr_group_rows_device", x, "x", plan.n, plan, weights, plan.n_ids, out, ctx)
 
 
+@_on_its_stream
 def group_grad(dout, plan: Plan, *, weights=None, x=None, out=None, ctx=None):
     """Gradients of ``group`` from that of its output: ``dx[i] = sum_c
     weights[i, c] * dout[slot[i, c]]`` and, where ``x`` is given, also that of
@@ -437,12 +428,14 @@ def group_grad(dout, plan: Plan, *, weights=None, x=None, out=None, ctx=None):
     return _token_grad("mvr_group_rows_grad_device", dout, plan.n_ids, plan, weights, x, "x", plan.n, plan.n, out, ctx)
 
 
+@_on_its_stream
 def ungroup(xs, plan: Plan, *, weights=None, out=None, ctx=None):
     """Sorted rows back to their tokens: ``out[i] = sum_c weights[i, c] *
     xs[slot[i, c]]``; zeros for a token none of whose ids names a row."""
     return _token_call("mvr_ungroup_rows_device", xs, "xs", plan.n_ids, plan, weights, plan.n, out, ctx)
 
 
+@_on_its_stream
 def ungroup_grad(dout, plan: Plan, *, weights=None, xs=None, out=None, ctx=None):
     """Gradients of ``ungroup`` from that of its output: ``dxs[slot[i, c]] =
     weights[i, c] * dout[i]`` (rows behind the last sorted one keep what
