@@ -16,7 +16,8 @@ namespace {
 // pair goes to (pairs of smaller digits) + (pairs of its digit before it). The
 // ids are a few bytes a token beside rows of hundreds, so what costs is the
 // number of dependent steps: some thousand pairs go through all passes in
-// one launch of one cluster of blocks; above, a pass is three launches over tiles.
+// one launch of one cluster of blocks; above, a pass is two or three launches
+// over tiles.
 
 constexpr int kMostBits = 10;  // of a digit
 constexpr uint32_t kSmallThreads = 256, kSmallRounds = 8, kSmallBlocks = 8;
@@ -203,6 +204,12 @@ plan_small_kernel(PlanArgs A, uint32_t rounds, int digit_bits, int passes, uint3
   }
 }
 
+// Up to so many tiles a scatter sums the counts of the tiles before it itself
+// (then hist is [tile][digit]), which saves a launch: 14.9 us for the plan of
+// 16,384 ids instead of 18.4, at 65,536 both take 19. Above, plan_scan_kernel
+// does it for all.
+constexpr uint32_t kDirectTiles = 64;
+
 // Pairs of each digit in a tile: hist[digit][tile].
 template <class I, uint32_t ROUNDS>
 __global__ void __launch_bounds__(kTileThreads)
@@ -224,7 +231,9 @@ plan_hist_kernel(const void* __restrict__ src, uint32_t n, uint32_t rows, int sh
   for (uint32_t j = 0; j < ROUNDS; ++j)
     if (first + j * kTileThreads < n) atomicAdd(&s_count[(key[j] >> shift) & (R - 1)], 1u);
   __syncthreads();
-  for (uint32_t d = t; d < R; d += kTileThreads) hist[(uint64_t)d * tiles + blockIdx.x] = s_count[d];
+  const bool direct = tiles <= kDirectTiles;
+  for (uint32_t d = t; d < R; d += kTileThreads)
+    hist[direct ? (uint64_t)blockIdx.x * R + d : (uint64_t)d * tiles + blockIdx.x] = s_count[d];
 }
 
 // A digit's counts become those of the tiles before; its total beside them.
@@ -284,7 +293,27 @@ plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __
     key[j] = q < in_tile ? key_at<I>(src, tile0 + q, A.rows) : 0;
   }
   for (uint32_t e = t; e < kWarps * R; e += kTileThreads) s_count[e] = 0;
-  for (uint32_t d = t; d < R; d += kTileThreads) s_glob[d] = total[d];
+  constexpr uint32_t kDigits = (1u << kMostBits) / kTileThreads;  // of a thread
+  uint32_t before[kDigits];  // the digit's pairs in the tiles before
+#pragma unroll
+  for (uint32_t k = 0; k < kDigits; ++k) {
+    const uint32_t d = t + k * kTileThreads;
+    before[k] = 0;
+    if (d >= R) break;
+    if (tiles <= kDirectTiles) {
+      uint32_t all = 0;
+#pragma unroll 8
+      for (uint32_t q = 0; q < tiles; ++q) {
+        const uint32_t x = hist[q * R + d];
+        before[k] += q < blockIdx.x ? x : 0;
+        all += x;
+      }
+      s_glob[d] = all;
+    } else {
+      before[k] = hist[(uint64_t)d * tiles + blockIdx.x];
+      s_glob[d] = total[d];
+    }
+  }
   __syncthreads();
   uint32_t* mine = s_count + warp * R;
 #pragma unroll
@@ -294,8 +323,11 @@ plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __
   for (uint32_t d = t; d < R; d += kTileThreads) s_start[d] = warps_prefix(s_count + d, R, kWarps);
   __syncthreads();
   block_prefix(s_start, R, kTileThreads, s_warp);
-  for (uint32_t d = t; d < R; d += kTileThreads)
-    s_glob[d] += hist[(uint64_t)d * tiles + blockIdx.x] - s_start[d];
+#pragma unroll
+  for (uint32_t k = 0; k < kDigits; ++k) {
+    const uint32_t d = t + k * kTileThreads;
+    if (d < R) s_glob[d] += before[k] - s_start[d];
+  }
 #pragma unroll
   for (uint32_t j = 0; j < ROUNDS; ++j) {
     const uint32_t d = (key[j] >> shift) & (R - 1);
@@ -490,7 +522,7 @@ int plan_pass_of(Ctx* c, const PlanArgs& A, const void* kin, const uint32_t* vin
   const size_t smem = (2 * R + std::max(kTileThreads / 32 * R, 2 * kTile)) * 4;  // 40 KB at most: needs no request
   const auto count = plan_hist_kernel<I, ROUNDS>;
   MVR_CUDA(c, launch_pdl(count, tiles, kTileThreads, 0, st, kin, A.n, A.rows, shift, R, tiles, hist));
-  MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
+  if (tiles > kDirectTiles) MVR_CUDA(c, launch_pdl(plan_scan_kernel, R, 256, 0, st, tiles, hist, sums));
   const auto scatter = last ? plan_scatter_kernel<I, ROUNDS, true> : plan_scatter_kernel<I, ROUNDS, false>;
   MVR_CUDA(c, launch_pdl(scatter, tiles, kTileThreads, smem, st, A, kin, vin, shift, bits, tiles, hist, sums, kout,
                          vout));
