@@ -472,6 +472,20 @@ def test_group_of_nothing():
     assert bool((y == 0).all())
 
 
+@pytest.mark.parametrize("n,columns,dim", [(40, 2, 64), (40, 4, 256), (40, 8, 64), (40, 12, 64), (3, 3, 5000), (3000, 4, 1024)])
+def test_dropped_choices_meet_no_infinity(n, columns, dim):
+    g = gen(n)
+    ids = make_ids(g, (n, columns), 9, pad=0.4)
+    p = tokens.plan(ids, 9)
+    drop = p.slot < 0
+    x = torch.full((n, dim), float("inf"), device="cuda")
+    rows = normal(g, n * columns, dim).abs() + 1
+    _, dw = tokens.group_grad(rows, p, x=x)
+    assert bool((dw[drop] == 0).all()) and bool((dw[~drop] == float("inf")).all())
+    dxs, dw = tokens.ungroup_grad(x, p, xs=rows)
+    assert bool((dw[drop] == 0).all()) and bool((dw[~drop] == float("inf")).all())
+
+
 def test_the_same_row_twice():
     # one token may choose one group several times: a place for each
     ids = torch.tensor([[2, 2, 2], [0, 2, 0]], device="cuda")
