@@ -7,4 +7,4 @@ in ``libmvr_b200.so`` (hand-written sm_100a CUDA behind the C ABI of
 """
 from ._lib import Context, MvrError, default_context, load  # noqa: F401
 
-__all__ = ["Context", "MvrError", "default_context", "load", "pq", "kmeans", "synth", "tokens"]
+__all__ = ["Context", "MvrError", "default_context", "load", "pq", "kmeans", "synth"]
