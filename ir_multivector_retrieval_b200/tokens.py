@@ -50,13 +50,36 @@ def _id_bytes(ids) -> int:
     return n
 
 
-def _rows(t, what: str, n: int | None = None, dim: int | None = None):
+def _ends(shape) -> set:
+    """Where the dimensions of a shape end, counted in elements from its last
+    dimension to the first: what splitting and merging dimensions keeps."""
+    ends, k = set(), 1
+    for d in reversed(shape):
+        k *= d
+        ends.add(k)
+    ends.discard(1)
+    return ends
+
+
+def _in_order(shape, of) -> bool:
+    """Whether values of shape `shape` stand for those of shape `of` one by one
+    in memory order: the same dimensions, some of them split or merged (flat
+    among them). A transposed shape has as many values, each beside the wrong
+    one. Both shapes have the same number of values."""
+    a, b = _ends(shape), _ends(of)
+    return 0 in a or a <= b or b <= a
+
+
+def _rows(t, what: str, n: int | None = None, dim: int | None = None, of=None):
     """`t` as a 2-D view (copied where its rows are not consecutive), its row
-    length and its row stride."""
+    length and its row stride. `of`: the shape of what its rows belong to."""
     if t.dim() != 2:
         if t.dim() < 2:
             _refuse(f"{what} must have rows: at least two dimensions", "DimMismatch")
+        lead = t.shape[:-1]
         t = t.reshape(-1, t.shape[-1])
+        if of is not None and lead != of and t.shape[0] == n and not _in_order(lead, of):
+            _refuse(f"{what} has rows in shape {tuple(lead)}, not {tuple(of)}", "LengthMismatch")
     m, d = t.shape
     if dim is not None and d != dim:
         _refuse(f"{what} has rows of {d}, not {dim}", "DimMismatch")
@@ -71,9 +94,9 @@ def _rows(t, what: str, n: int | None = None, dim: int | None = None):
     return t, d, stride if m > 1 else d
 
 
-def _out_rows(t, what: str, n: int, dim: int, dtype):
+def _out_rows(t, what: str, n: int, dim: int, dtype, of=None):
     """Address and row stride of an output given by the caller: written in
-    place, so never copied."""
+    place, so never copied. `of`: the shape of what its rows belong to."""
     if t.dtype != dtype:
         _refuse(f"{what} must be {dtype}, not {t.dtype}")
     if t.dim() < 2 or t.shape[-1] != dim:
@@ -81,6 +104,8 @@ def _out_rows(t, what: str, n: int, dim: int, dtype):
     if t.numel() != n * dim:
         _refuse(f"{what} must have {n} rows of {dim}", "OutBufferWrongSize")
     if t.dim() > 2:
+        if of is not None and t.shape[:-1] != of and not _in_order(t.shape[:-1], of):
+            _refuse(f"{what} must have {dim} elements for each id of {tuple(of)}", "OutBufferWrongSize")
         try:
             t = t.view(n, dim)
         except RuntimeError:
@@ -91,11 +116,15 @@ def _out_rows(t, what: str, n: int, dim: int, dtype):
     return t.data_ptr(), stride if n > 1 else dim
 
 
-def _f32(t, n: int, what: str):
+def _f32(t, n: int, of, what: str):
+    """`t` with one value for each of the n ids of shape `of`."""
     if t.dtype != _F32:
         _refuse(f"{what} must be float32, not {t.dtype}")
-    if t.numel() != n:
-        _refuse(f"{what} has {t.numel()} values, not {n}", "LengthMismatch")
+    if t.shape != of:
+        if t.numel() != n:
+            _refuse(f"{what} has {t.numel()} values, not {n}", "LengthMismatch")
+        if not _in_order(t.shape, of):
+            _refuse(f"{what} has shape {tuple(t.shape)}, not {tuple(of)}", "LengthMismatch")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -303,7 +332,9 @@ def plan(ids, rows: int, *, ctx=None) -> Plan:
 def lookup(table, ids, *, scale=None, alpha: float = 1.0, out=None, ctx=None):
     """``out[i] = (alpha * scale[i]) * table[ids[i]]``: the ids' shape plus the
     table's row length, in the table's type; zero rows where an id names none.
-    ``scale`` (the ids' shape, f32) and ``out`` are optional."""
+    ``scale`` (the ids' shape, f32) and ``out`` are optional. What has the ids'
+    shape here and below may have its dimensions split or merged, flat for
+    instance; another shape of as many values is refused."""
     dt = _dtype(table, "table")
     idb = _id_bytes(ids)
     n = ids.numel()
@@ -314,12 +345,12 @@ def lookup(table, ids, *, scale=None, alpha: float = 1.0, out=None, ctx=None):
     table, dim, ts = _rows(table, "table")
     flat = ids.contiguous()
     if scale is not None:
-        scale = _f32(scale, n, "scale")
+        scale = _f32(scale, n, ids.shape, "scale")
     if out is None:
         out = table.new_empty((*ids.shape, dim))
         po, so = out.data_ptr(), dim
     else:
-        po, so = _out_rows(out, "out", n, dim, table.dtype)
+        po, so = _out_rows(out, "out", n, dim, table.dtype, ids.shape)
     _run(ctx, device, "mvr_lookup_device", table.data_ptr(), dt, rows, dim, ts, flat.data_ptr(), idb, n, _ptr(scale),
          alpha, po, so)
     return out
@@ -341,9 +372,9 @@ def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None,
     if accumulate and out is None:
         _refuse("accumulate needs out")
     device = _device_of(grad, plan.offsets, plan.order, plan.keys, plan.slot, scale, table, out)
-    grad, dim, gs = _rows(grad, "grad", n)
+    grad, dim, gs = _rows(grad, "grad", n, None, plan.slot.shape)
     if scale is not None:
-        scale = _f32(scale, n, "scale")
+        scale = _f32(scale, n, plan.slot.shape, "scale")
     tp, ts, dscale = None, dim, None
     if table is not None:
         if table.dtype != grad.dtype:
@@ -375,7 +406,7 @@ def _token_call(name: str, src, what: str, from_n: int, plan: Plan, weights, to_
     device = _device_of(src, slot, weights, out)
     src, dim, ss = _rows(src, what, from_n)
     if weights is not None:
-        weights = _f32(weights, n_ids, "weights")
+        weights = _f32(weights, n_ids, slot.shape, "weights")
     if out is None:
         out = src.new_empty((to_n, dim))
         po, so = out.data_ptr(), dim
@@ -394,7 +425,7 @@ def _token_grad(name: str, src, from_n: int, plan: Plan, weights, other, other_w
     device = _device_of(src, slot, weights, other, out)
     src, dim, ss = _rows(src, "dout", from_n)
     if weights is not None:
-        weights = _f32(weights, n_ids, "weights")
+        weights = _f32(weights, n_ids, slot.shape, "weights")
     dw, op, os_ = None, None, dim
     if other is not None:
         if other.dtype != src.dtype:

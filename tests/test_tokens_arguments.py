@@ -1,0 +1,78 @@
+"""What the token operators make of their arguments, without a GPU: host
+tensors stand for device tensors and the library's calls are only noted."""
+import pytest
+import torch
+
+from ir_multivector_retrieval_b200 import tokens
+from ir_multivector_retrieval_b200._lib import MvrError
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+    monkeypatch.setattr(tokens, "_device_of", lambda *t: 0)
+    monkeypatch.setattr(tokens, "_run", lambda ctx, device, name, *args: made.append(name))
+    return made
+
+
+def _plan(*shape, rows=8):
+    n = torch.Size(shape).numel()
+    i32 = torch.int32
+    return tokens.Plan(rows, torch.zeros(rows + 1, dtype=i32), torch.arange(n, dtype=i32), torch.zeros(n, dtype=i32),
+                       torch.arange(n, dtype=i32).view(shape))
+
+
+def _refused(calls, fn, *a, **k):
+    with pytest.raises(MvrError) as e:
+        fn(*a, **k)
+    assert not calls  # nothing was launched
+    return e.value.name
+
+
+# ---- shapes: as many values in another order are not the ids' --------------------
+
+OTHER = [((6, 4), (4, 6)), ((6, 4), (2, 12)), ((2, 6), (6, 2)), ((3, 1, 5), (5, 3)), ((2, 3, 4), (4, 3, 2)),
+         ((2, 3, 4), (2, 4, 3)), ((2, 3, 4), (3, 2, 4))]
+SAME = [((6, 4), (6, 4)), ((6, 4), (24,)), ((24,), (6, 4)), ((6, 4), (2, 3, 4)), ((6, 4), (6, 1, 4)), ((6,), (6, 1)),
+        ((6,), (1, 6)), ((6, 1), (1, 6)), ((1,), ()), ((), (1, 1)), ((2, 3, 4), (6, 4)), ((0, 4), (4, 0)), ((5, 0), (0,))]
+
+
+@pytest.mark.parametrize("ids,got", OTHER)
+def test_values_in_another_order_are_refused(calls, ids, got):
+    t, n = torch.zeros(8, 16), torch.Size(ids).numel()
+    i = torch.zeros(ids, dtype=torch.int32)
+    assert _refused(calls, tokens.lookup, t, i, scale=torch.zeros(got)) == "LengthMismatch"
+    assert _refused(calls, tokens.lookup, t, i, out=torch.zeros(*got, 16)) == "OutBufferWrongSize"
+    p = _plan(*ids)
+    grad = torch.zeros(n, 16)
+    assert _refused(calls, tokens.lookup_grad, grad, p, scale=torch.zeros(got)) == "LengthMismatch"
+    assert _refused(calls, tokens.lookup_grad, torch.zeros(*got, 16), p) == "LengthMismatch"
+    w, x, xs = torch.zeros(got), torch.zeros(p.n, 16), torch.zeros(n, 16)
+    for fn, a in ((tokens.group, x), (tokens.ungroup, xs), (tokens.group_grad, xs), (tokens.ungroup_grad, x)):
+        assert _refused(calls, fn, a, p, weights=w) == "LengthMismatch"
+
+
+def test_transposed_weights_are_refused(calls):
+    p = _plan(6, 4)
+    w = torch.zeros(6, 4)
+    tokens.group(torch.zeros(6, 16), p, weights=w)
+    calls.clear()
+    assert _refused(calls, tokens.group, torch.zeros(6, 16), p, weights=w.t()) == "LengthMismatch"
+    # one value a token is not one a choice
+    assert _refused(calls, tokens.group, torch.zeros(6, 16), p, weights=torch.zeros(6)) == "LengthMismatch"
+
+
+@pytest.mark.parametrize("ids,got", SAME)
+def test_values_in_the_ids_order_are_taken(calls, ids, got):
+    t, n = torch.zeros(8, 16), torch.Size(ids).numel()
+    i = torch.zeros(ids, dtype=torch.int32)
+    out = torch.zeros(*got, 16) if got else torch.zeros(1, 16)
+    assert tokens.lookup(t, i, scale=torch.zeros(got), out=out) is out
+    if ids:
+        p = _plan(*ids)
+        grad = torch.zeros(*got, 16) if got else torch.zeros(1, 16)
+        tokens.lookup_grad(grad, p, scale=torch.zeros(got), table=t)
+        if len(ids) > 1 and n:
+            tokens.group(torch.zeros(p.n, 16), p, weights=torch.zeros(got))
+            tokens.ungroup_grad(torch.zeros(p.n, 16), p, weights=torch.zeros(got), xs=torch.zeros(n, 16))
+    assert calls
