@@ -10,7 +10,13 @@ All tensors are torch tensors on one GPU: rows f32, bf16 or f16, ids int32,
 int64 or uint32, scales and weights f32. Ids outside [0, rows), negative ones
 among them, name no row. The calls enqueue on the stream given to
 ``ctx.set_stream``, else on torch's current stream, and return without
-waiting; they may be captured into a CUDA graph. There is no CPU fallback.
+waiting; after one ordinary call on the GPU they may be captured into a CUDA
+graph. There is no CPU fallback.
+
+No autograd graph is made: results are detached, also where an input requires
+a gradient, and the gradients are calls of their own. A tensor given as
+``out`` counts as changed in place, so a graph that saved what it held before
+is refused by ``backward``. Inputs and outputs of a call must not overlap.
 """
 from __future__ import annotations
 
@@ -21,6 +27,7 @@ import threading
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.graph import increment_version as _written
 
 from . import _lib
 from ._lib import CODES, MvrError
@@ -346,6 +353,7 @@ def lookup(table, ids, *, scale=None, alpha: float = 1.0, out=None, ctx=None):
     flat = ids.contiguous()
     if scale is not None:
         scale = _f32(scale, n, ids.shape, "scale")
+    given = out
     if out is None:
         out = table.new_empty((*ids.shape, dim))
         po, so = out.data_ptr(), dim
@@ -353,6 +361,8 @@ def lookup(table, ids, *, scale=None, alpha: float = 1.0, out=None, ctx=None):
         po, so = _out_rows(out, "out", n, dim, table.dtype, ids.shape)
     _run(ctx, device, "mvr_lookup_device", table.data_ptr(), dt, rows, dim, ts, flat.data_ptr(), idb, n, _ptr(scale),
          alpha, po, so)
+    if given is not None:
+        _written(given)
     return out
 
 
@@ -382,6 +392,7 @@ def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None,
         table, _, ts = _rows(table, "table", rows, dim)
         tp = table.data_ptr()
         dscale = grad.new_empty(plan.slot.shape, dtype=_F32)
+    given = out
     if out is None:
         out = grad.new_empty((rows, dim))
         po, so, odt = out.data_ptr(), dim, dt
@@ -395,6 +406,8 @@ def lookup_grad(grad, plan: Plan, *, scale=None, alpha: float = 1.0, table=None,
     _run(ctx, device, "mvr_lookup_grad_device", grad.data_ptr(), dt, gs, n, rows, dim, plan.offsets.data_ptr(),
          plan.order.data_ptr(), plan.keys.data_ptr(), _ptr(scale), alpha, tp, ts, po, odt, so, int(accumulate),
          _ptr(dscale), _ptr(ws), need)
+    if given is not None:
+        _written(given)
     return out if dscale is None else (out, dscale)
 
 
@@ -407,12 +420,15 @@ def _token_call(name: str, src, what: str, from_n: int, plan: Plan, weights, to_
     src, dim, ss = _rows(src, what, from_n)
     if weights is not None:
         weights = _f32(weights, n_ids, slot.shape, "weights")
+    given = out
     if out is None:
         out = src.new_empty((to_n, dim))
         po, so = out.data_ptr(), dim
     else:
         po, so = _out_rows(out, "out", to_n, dim, src.dtype)
     _run(ctx, device, name, src.data_ptr(), dt, ss, plan.n, plan.columns, dim, slot.data_ptr(), _ptr(weights), po, so)
+    if given is not None:
+        _written(given)
     return out
 
 
@@ -433,6 +449,7 @@ def _token_grad(name: str, src, from_n: int, plan: Plan, weights, other, other_w
         other, _, os_ = _rows(other, other_what, other_n, dim)
         op = other.data_ptr()
         dw = src.new_empty(slot.shape, dtype=_F32)
+    given = out
     if out is None:
         out = src.new_empty((to_n, dim))
         po, so = out.data_ptr(), dim
@@ -440,6 +457,8 @@ def _token_grad(name: str, src, from_n: int, plan: Plan, weights, other, other_w
         po, so = _out_rows(out, "out", to_n, dim, src.dtype)
     _run(ctx, device, name, src.data_ptr(), dt, ss, plan.n, plan.columns, dim, slot.data_ptr(), _ptr(weights), op, os_,
          po, so, _ptr(dw))
+    if given is not None:
+        _written(given)
     return out if dw is None else (out, dw)
 
 

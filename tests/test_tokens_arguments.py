@@ -76,3 +76,44 @@ def test_values_in_the_ids_order_are_taken(calls, ids, got):
             tokens.group(torch.zeros(p.n, 16), p, weights=torch.zeros(got))
             tokens.ungroup_grad(torch.zeros(p.n, 16), p, weights=torch.zeros(got), xs=torch.zeros(n, 16))
     assert calls
+
+
+# ---- outputs given by the caller ---------------------------------------------------
+
+def _writes(rows, dim):
+    """Every call that takes an output, with the shape of that output."""
+    i, p = torch.zeros(6, dtype=torch.int32), _plan(6, 2)
+    q, t = _plan(6), torch.zeros(rows, dim)
+    x, xs = torch.zeros(6, dim), torch.zeros(12, dim)
+    return [(lambda o: tokens.lookup(t, i, out=o), 6), (lambda o: tokens.lookup_grad(x, q, out=o), rows),
+            (lambda o: tokens.lookup_grad(x, q, table=t, out=o, accumulate=True), rows),
+            (lambda o: tokens.group(x, p, out=o), 12), (lambda o: tokens.ungroup(xs, p, out=o), 6),
+            (lambda o: tokens.group_grad(xs, p, out=o), 6), (lambda o: tokens.group_grad(xs, p, x=x, out=o), 6),
+            (lambda o: tokens.ungroup_grad(x, p, out=o), 12), (lambda o: tokens.ungroup_grad(x, p, xs=xs, out=o), 12)]
+
+
+@pytest.mark.parametrize("k", range(9))
+def test_an_output_counts_as_changed(calls, k):
+    call, n = _writes(8, 16)[k]
+    out = torch.zeros(n, 16)
+    leaf = torch.ones(n, 16, requires_grad=True)
+    loss = (leaf * out).sum()  # saves what out holds
+    call(out)
+    assert calls
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    wide = torch.zeros(n, 40)  # a view counts for its base
+    before = wide._version
+    call(wide[:, 3:19])
+    assert wide._version > before
+    with torch.inference_mode():
+        call(torch.zeros(n, 16))
+
+
+def test_inputs_do_not_count_as_changed(calls):
+    for call, n in _writes(8, 16):
+        closed = {k: v for k, v in zip(call.__code__.co_freevars, (c.cell_contents for c in call.__closure__))}
+        tensors = [v for v in closed.values() if isinstance(v, torch.Tensor)]
+        before = [t._version for t in tensors]
+        call(torch.zeros(n, 16))
+        assert [t._version for t in tensors] == before
