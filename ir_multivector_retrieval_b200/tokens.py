@@ -83,6 +83,8 @@ def _rows(t, what: str, n: int | None = None, dim: int | None = None, of=None):
     if t.dim() != 2:
         if t.dim() < 2:
             _refuse(f"{what} must have rows: at least two dimensions", "DimMismatch")
+        if t.shape[-1] == 0:
+            _refuse(f"{what} has rows of length 0", "DimMismatch")
         lead = t.shape[:-1]
         t = t.reshape(-1, t.shape[-1])
         if of is not None and lead != of and t.shape[0] == n and not _in_order(lead, of):

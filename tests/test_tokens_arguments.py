@@ -117,3 +117,10 @@ def test_inputs_do_not_count_as_changed(calls):
         before = [t._version for t in tensors]
         call(torch.zeros(n, 16))
         assert [t._version for t in tensors] == before
+
+
+@pytest.mark.parametrize("shape", [(6, 0), (2, 3, 0), (0, 3, 0)])
+def test_rows_of_no_length_are_refused(calls, shape):
+    p = _plan(shape[0] if len(shape) == 2 else shape[0] * shape[1])
+    for fn in (tokens.lookup_grad, tokens.group, tokens.ungroup, tokens.group_grad, tokens.ungroup_grad):
+        assert _refused(calls, fn, torch.zeros(shape), p) == "DimMismatch"
