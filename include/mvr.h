@@ -681,10 +681,13 @@ int mvr_normalize_rows_device(mvr_ctx* ctx, float* d_rows, uint64_t n_floats, ui
  *
  * Rows have `dim` elements of one type (mvr_dtype), consecutive inside a row;
  * `*_stride` is the distance of two rows in elements (at least dim for
- * outputs, any value for inputs: 0 repeats one row; below 2^32). Scales and weights are
- * f32. Sums and products are formed in f32 and rounded once to the element
- * type. Results do not depend on the launch: the order of every sum is fixed
- * by the sizes.
+ * outputs, any value for inputs: 0 repeats one row; below 2^32 for both).
+ * Scales and weights are f32. Sums and products are formed in f32 and rounded
+ * once to the element type. No sum is formed by atomics: the same call gives
+ * the same bits each time on one kind of GPU. The order of a sum follows from
+ * the sizes, types, strides and address alignments of the call and the number
+ * of SMs, so another layout of any operand (a table or xs that is read for the
+ * second gradient alone, an output at another alignment) may change last bits.
  *
  * Ids are 4-byte (id_bytes = 4) or 8-byte integers. An id outside [0, rows),
  * a negative one among them, names no row (padding, a dropped choice): its

@@ -14,7 +14,7 @@ namespace {
 // them a thread, the block's stride apart, when there is work for all SMs. All
 // ids and scales are asked for before the first is used: the chain from an id
 // to its row is what a block's time consists of. 1,521,797 x 64 f32 from 32,768
-// rows with scales: 73 us (5.6 TB/s) with two accesses of 32 bytes a thread and
+// rows with scales: 71 us (5.6 TB/s) with two accesses of 32 bytes a thread and
 // eight blocks an SM, 81 us with four of 16 bytes and six, 93 with eight.
 template <class T, class I, int V, int UR, bool SCALE>
 __global__ void __launch_bounds__(256, sizeof(T) * V == 32 ? 8 : 6)
@@ -82,12 +82,11 @@ int lookup_run(Ctx* c, uint64_t n, uint32_t chunks, const void* table, uint64_t 
 // places, which costs no more than reading it in order; the scale's gradient
 // comes out of the same pass (its own would read the gradient again). At
 // 1,521,797 x 64 f32 over 32,768 rows, a seventh of the tokens in one of them:
-// 82 us (4.8 TB/s of gradient), 100 us with the scale's gradient (75 and 83 us
-// of it the tiles at uniform ids, the rest the joining launch and, where short
-// keys meet in a block, groups that wait for one another). Rows through a ring
-// of asynchronous copies in shared memory, 32 bytes a lane, eight rows in
-// flight, 128 threads a block and groups of 32 or 128 places measured no
-// faster.
+// 86 us (4.5 TB/s of gradient), 101 us with the scale's gradient: the tiles, the
+// joining launch and, where short keys meet in a block, groups that wait for one
+// another. Rows through a ring of asynchronous copies in shared memory, 32 bytes
+// a lane, eight rows in flight, 128 threads a block and groups of 32 or 128
+// places measured no faster.
 
 // Chunks a lane holds: 16 bytes of a row, in several pieces where its length or
 // alignment does not allow one.

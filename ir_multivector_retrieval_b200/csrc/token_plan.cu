@@ -264,9 +264,10 @@ plan_scan_kernel(uint32_t tiles, uint32_t* __restrict__ hist, uint32_t* __restri
 }
 
 // A tile's pairs, sorted by digit in shared memory first so that each digit's
-// run is written in one piece. At 1,521,797 pairs blocks of 256 threads that
-// share an SM by fours measured best (the plan 51 us; 54 with six or with
-// blocks of 512 threads by twos, 70 with one of 1024).
+// run is written in one piece. Blocks of 256 threads that share an SM by fours
+// measured best: the plan of 1,521,797 pairs over 32,768 rows takes 48 us, 7 %
+// more with six of them, 4 % more with blocks of 512 threads by twos (the same
+// at 800,000 and 3,000,000 pairs).
 template <class I, uint32_t ROUNDS, bool LAST>
 __global__ void __launch_bounds__(kTileThreads, 4)
 plan_scatter_kernel(PlanArgs A, const void* __restrict__ src, const uint32_t* __restrict__ vin, int shift,
@@ -457,12 +458,24 @@ struct Digits {
   }
 };
 
-// Whether one cluster does it: a pass takes it as long as the tiles' three
-// launches at some 10,000 pairs.
+// Whether one cluster does it. A pass takes it as long as the tiles' two
+// launches at some 7,000 pairs: over 32,768 rows 15.2 us against 17.6 at 6,000
+// pairs, 17.2 against 14.8 at 8,193 (three passes, 3,000,000 rows: 40 against
+// 43, 44 against 42). A single pass has the offsets beside it, which the tiles
+// need another launch for: over 800 rows 12.3 against 14.3 us at 12,000 pairs,
+// 13.9 against 12.3 at 16,384, the most the cluster holds.
 bool is_small(uint64_t n, const Digits& D) { return n <= (D.passes == 1 ? kSmallMax : kSmallMaxPasses); }
 
-// Pairs a thread of a tile: few until the blocks are more than share the SMs
-// (then the most that 64 registers hold: 47 us at 1,521,797 pairs, with 8 50).
+// Pairs a thread of a tile: few while the tiles are one wave of four blocks an
+// SM, then the most that 64 registers hold. Few give more blocks to wait at
+// once, many fewer counts to sum and longer runs to write; the plan over 1,000 /
+// 32,768 / 1,000,000 rows in us:
+//   450,000 pairs    4 each: 22 / 27 / 43    11 each: 25 / 33 / 48
+//   606,209          27 / 31 / 51            25 / 34 / 48
+//   800,000          33 / 37 / 64            27 / 35 / 50
+//   1,521,797        53 / 57 / 102           37 / 49 / 70
+// A workspace is asked for without a device at hand, so the SMs are a number
+// here: those of a B200.
 constexpr uint32_t kFewRounds = 4, kManyRounds = 11;
 bool few_rounds(uint64_t n) { return n <= 148ull * 4 * kFewRounds * kTileThreads; }
 

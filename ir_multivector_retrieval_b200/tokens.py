@@ -7,11 +7,12 @@ grouping (``group``, ``ungroup``) read it. A group is any id below ``rows``:
 the expert a router chose, the centroid ``tac.cluster_flat`` assigned.
 
 All tensors are torch tensors on one GPU: rows f32, bf16 or f16, ids int32,
-int64 or uint32, scales and weights f32. Ids outside [0, rows), negative ones
-among them, name no row. The calls enqueue on the stream given to
-``ctx.set_stream``, else on torch's current stream, and return without
-waiting; after one ordinary call on the GPU they may be captured into a CUDA
-graph. There is no CPU fallback.
+int64 or uint32, scales and weights f32. Inputs whose rows are not consecutive
+inside are copied first; rows 2^32 and more elements apart are refused. Ids
+outside [0, rows), negative ones among them, name no row. The calls enqueue on
+the stream given to ``ctx.set_stream``, else on torch's current stream, and
+return without waiting; after one ordinary call on the GPU they may be captured
+into a CUDA graph. There is no CPU fallback.
 
 No autograd graph is made: results are detached, also where an input requires
 a gradient, and the gradients are calls of their own. A tensor given as
