@@ -8,11 +8,11 @@ the expert a router chose, the centroid ``tac.cluster_flat`` assigned.
 
 All tensors are torch tensors on one GPU: rows f32, bf16 or f16, ids int32,
 int64 or uint32, scales and weights f32. Inputs whose rows are not consecutive
-inside are copied first; rows 2^32 and more elements apart are refused. Ids
-outside [0, rows), negative ones among them, name no row. The calls enqueue on
-the stream given to ``ctx.set_stream``, else on torch's current stream, and
-return without waiting; after one ordinary call on the GPU they may be captured
-into a CUDA graph. There is no CPU fallback.
+inside, or 2^32 and more elements apart, are copied first; such outputs are
+refused. Ids outside [0, rows), negative ones among them, name no row. The
+calls enqueue on the stream given to ``ctx.set_stream``, else on torch's
+current stream, and return without waiting; after one ordinary call on the GPU
+they may be captured into a CUDA graph. There is no CPU fallback.
 
 No autograd graph is made: results are detached, also where an input requires
 a gradient, and the gradients are calls of their own. A tensor given as
@@ -79,8 +79,10 @@ def _in_order(shape, of) -> bool:
 
 
 def _rows(t, what: str, n: int | None = None, dim: int | None = None, of=None):
-    """`t` as a 2-D view (copied where its rows are not consecutive), its row
-    length and its row stride. `of`: the shape of what its rows belong to."""
+    """`t` as a 2-D view, its row length and its row stride. Copied where its
+    rows are not consecutive inside or 2^32 and more elements apart, which the
+    library refuses: such rows are few. `of`: the shape of what its rows belong
+    to."""
     if t.dim() != 2:
         if t.dim() < 2:
             _refuse(f"{what} must have rows: at least two dimensions", "DimMismatch")
@@ -98,7 +100,7 @@ def _rows(t, what: str, n: int | None = None, dim: int | None = None, of=None):
     if d == 0:
         _refuse(f"{what} has rows of length 0", "DimMismatch")
     stride, one = t.stride()
-    if one != 1 and d > 1:
+    if one != 1 and d > 1 or stride >> 32 and m > 1:
         t = t.contiguous()
         stride = d
     return t, d, stride if m > 1 else d

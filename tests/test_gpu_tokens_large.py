@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from ir_multivector_retrieval_b200 import tokens
+from ir_multivector_retrieval_b200._lib import MvrError
 from test_gpu_tokens import BF16, F16, F32, TINY, U, U32, gen, lookup_grad_check, lookup_ref, make_ids, normal, plan_of, within
 
 pytestmark = pytest.mark.gpu
@@ -148,3 +149,66 @@ def test_group_and_back(dtype, n, columns, dim, weighted):
     dx, dw = tokens.group_grad(rows, p, weights=w, x=x)
     within(dx, want, tol)
     within(dw, of, off)
+
+
+def test_inputs_2_to_the_32_apart():
+    stride, dim = 2**32 + 8, 24
+    buf = torch.zeros(2 * stride + dim, dtype=BF16, device="cuda")
+    far = buf.as_strided((3, dim), (stride, 1))
+    near = normal(gen(7), 3, dim, dtype=BF16)
+    far.copy_(near)
+    ids = torch.tensor([2, 0, 1], device="cuda")
+    p = tokens.plan(ids, 3)
+    assert torch.equal(tokens.lookup(far, ids), near[ids])
+    dt, ds = tokens.lookup_grad(far, p, table=far)
+    wt, ws = tokens.lookup_grad(near, p, table=near)
+    assert torch.equal(dt, wt) and torch.equal(ds, ws)
+    assert torch.equal(tokens.group(far, p), tokens.group(near, p))
+    assert torch.equal(tokens.ungroup(far, p), tokens.ungroup(near, p))
+    for fn, kw in ((tokens.group_grad, "x"), (tokens.ungroup_grad, "xs")):
+        for a, b in zip(fn(far, p, **{kw: far}), fn(near, p, **{kw: near})):
+            assert torch.equal(a, b)
+    with pytest.raises(MvrError) as e:  # an output is written in place
+        tokens.lookup(near, ids, out=far)
+    assert e.value.name == "InvalidArgument" and torch.equal(far, near)
+
+
+# ---- shapes ----------------------------------------------------------------------------
+
+def test_shapes_split_merged_and_transposed():
+    g = gen(9)
+    b, c, k, rows, dim = 6, 5, 4, 30, 48
+    ids = make_ids(g, (b * c, k), rows, pad=0.1)
+    p = tokens.plan(ids, rows)
+    x, w = normal(g, b * c, dim), torch.rand(b * c, k, generator=g, device="cuda")
+    want = tokens.ungroup(tokens.group(x, p, out=torch.zeros(b * c * k, dim, device="cuda")), p, weights=w)
+    xs = tokens.group(x.view(b, c, dim), p, out=torch.zeros(b * c * k, dim, device="cuda"))
+    for same in (w.view(b, c, k), w.view(-1), w.t().contiguous().t(), w.view(b * c, 1, k)):
+        assert torch.equal(tokens.ungroup(xs, p, weights=same), want)
+    for other in (w.t(), w.view(b, c, k).transpose(0, 2), w.view(k, b * c)):
+        with pytest.raises(MvrError) as e:
+            tokens.ungroup(xs, p, weights=other)
+        assert e.value.name == "LengthMismatch"
+    table, grad = normal(g, rows, dim), normal(g, b * c, k, dim)
+    want = tokens.lookup(table, ids, scale=w)
+    out = torch.zeros(b, c, k, dim, device="cuda")
+    assert torch.equal(tokens.lookup(table, ids, scale=w.view(b, c, k), out=out).view_as(want), want)
+    dt, ds = tokens.lookup_grad(grad.view(b, c, k, dim), p, scale=w.view(-1), table=table)
+    wt, ws = tokens.lookup_grad(grad, p, scale=w, table=table)
+    assert torch.equal(dt, wt) and torch.equal(ds, ws)
+    for call in (lambda: tokens.lookup(table, ids, scale=w.t()),
+                 lambda: tokens.lookup_grad(grad.transpose(0, 1), p), lambda: tokens.lookup_grad(grad, p, scale=w.t())):
+        with pytest.raises(MvrError) as e:
+            call()
+        assert e.value.name == "LengthMismatch"
+
+
+def test_an_output_counts_as_changed():
+    g = gen(10)
+    table, ids = normal(g, 9, 16), make_ids(g, (7,), 9)
+    out = torch.zeros(7, 16, device="cuda")
+    leaf = torch.ones(7, 16, device="cuda", requires_grad=True)
+    loss = (leaf * out).sum()
+    tokens.lookup(table, ids, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

@@ -124,3 +124,15 @@ def test_rows_of_no_length_are_refused(calls, shape):
     p = _plan(shape[0] if len(shape) == 2 else shape[0] * shape[1])
     for fn in (tokens.lookup_grad, tokens.group, tokens.ungroup, tokens.group_grad, tokens.ungroup_grad):
         assert _refused(calls, fn, torch.zeros(shape), p) == "DimMismatch"
+
+
+# ---- strides -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("stride", [2**32 - 1, 2**32, 2**40])
+def test_inputs_far_apart_are_copied(calls, stride):
+    # without memory: the library takes strides below 2^32
+    far = torch.empty(1, device="meta").as_strided((3, 16), (stride, 1))
+    t, dim, got = tokens._rows(far, "x")
+    assert t.shape == (3, 16) and dim == 16 and got == (stride if stride < 2**32 else 16) and t.stride(0) == got
+    one, _, got = tokens._rows(far[:1], "x")
+    assert one.data_ptr() == far.data_ptr() and got == 16  # a single row has no stride to copy for
